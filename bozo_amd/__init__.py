@@ -7,5 +7,7 @@ bozo_amd/lib/libtension_hip.so), bound with ctypes under torch autograd.
 """
 from .ops import (TensionDecodeCache, causal_tension, decode_step, global_tension,  # noqa: F401
                   rope)
+from .paged import PagedKV, paged_append, paged_decode, paged_read  # noqa: F401
 
-__all__ = ["causal_tension", "global_tension", "decode_step", "TensionDecodeCache", "rope"]
+__all__ = ["causal_tension", "global_tension", "decode_step", "TensionDecodeCache", "rope",
+           "PagedKV", "paged_append", "paged_read", "paged_decode"]

@@ -19,6 +19,7 @@ HOST_PATH = os.path.join(_HERE, "lib", "_host.so")
 
 # dtype codes (enum in tension_hip.h)
 F32, BF16, F16, F64 = 0, 1, 2, 3
+E4M3, U8 = 4, 5  # pages of a paged cache and their exponent bytes
 DTYPE_CODE = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16, torch.float64: F64}
 
 # flags
@@ -45,7 +46,14 @@ class TensionBuf(ctypes.Structure):
                 ("reserved", ctypes.c_int32), ("s", ctypes.c_int64 * 4)]
 
 
+class TensionPaged(ctypes.Structure):
+    _fields_ = [("k", TensionBuf), ("v", TensionBuf), ("k_exp", TensionBuf), ("v_exp", TensionBuf),
+                ("table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("table_len", ctypes.c_int64),
+                ("pages", ctypes.c_int64), ("page_size", ctypes.c_int64)]
+
+
 BufP = ctypes.POINTER(TensionBuf)
+PagedP = ctypes.POINTER(TensionPaged)
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int32
 _f64 = ctypes.c_double
@@ -72,6 +80,10 @@ SIGNATURES = {
     "tension_aux_loss_fwd": (_i32, [BufP, _i32] + [_i64] * 4 + [_vp, _vp]),
     "tension_aux_loss_bwd": (_i32, [BufP, BufP, _i32] + [_i64] * 4 + [_vp, _vp]),
     "tension_bias_build": (_i32, [_vp, _i64, _i64, _i64, _vp, _vp, _i32, _f64, BufP, _vp, _vp]),
+    "tension_paged_append": (_i32, [PagedP, BufP, BufP, _vp, _vp] + [_i64] * 4 + [_vp]),
+    "tension_paged_read": (_i32, [PagedP, BufP, BufP, _vp, _vp] + [_i64] * 4 + [_vp]),
+    "tension_paged_decode_workspace": (_i64, [_i64] * 8),
+    "tension_paged_decode": (_i32, [PagedP, BufP, BufP, _vp, _vp] + [_i64] * 6 + [_f64, _i32, _vp]),
     "tension_last_error": (ctypes.c_char_p, []),
     "tension_version": (ctypes.c_char_p, []),
     "tension_last_kernel": (_i32, []),

@@ -776,6 +776,141 @@ int tension_aux_loss_bwd(const tension_buf* taus, const tension_buf* dtaus, int3
   return launched(e, "tension_aux_loss_bwd");
 }
 
+namespace {
+
+bool page_dtype(int dt) { return dt == TENSION_F32 || dt == TENSION_BF16 || dt == TENSION_F16 || dt == TENSION_E4M3; }
+
+int check_pages(const tension_buf& b, const tension_buf& e, const char* what) {
+  if (!b.ptr) return fail(TENSION_ERR_ARG, "%s: null data pointer", what);
+  if (!page_dtype(b.dtype)) return fail(TENSION_ERR_ARG, "%s: bad dtype code %d", what, b.dtype);
+  if (b.s[3] != 1)
+    return fail(TENSION_ERR_ARG, "%s: innermost stride must be 1 (got %lld)", what, (long long)b.s[3]);
+  if ((b.dtype == TENSION_E4M3) != (e.ptr != nullptr))
+    return fail(TENSION_ERR_ARG, "%s: exponent bytes belong to e4m3 pages, and to them only", what);
+  if (e.ptr && e.dtype != TENSION_U8) return fail(TENSION_ERR_ARG, "%s: exponents must be bytes", what);
+  return 0;
+}
+
+int check_paged(const tension_paged* c, PagedCache* out) {
+  if (!c) return fail(TENSION_ERR_ARG, "cache is required");
+  TRY(check_pages(c->k, c->k_exp, "k pages"));
+  TRY(check_pages(c->v, c->v_exp, "v pages"));
+  if (!c->table) return fail(TENSION_ERR_ARG, "table is required");
+  if (c->pages < 1 || c->pages > 0x7fffffff || c->page_size < 1 || c->page_size > 0x3fffffff || c->table_len < 0 ||
+      c->table_len > 0x7fffffff)
+    return fail(TENSION_ERR_ARG, "paged: bad sizes pages=%lld page_size=%lld table_len=%lld", (long long)c->pages,
+                (long long)c->page_size, (long long)c->table_len);
+  out->k = make_buf(&c->k); out->v = make_buf(&c->v);
+  out->ke = (const uint8_t*)c->k_exp.ptr; out->ve = (const uint8_t*)c->v_exp.ptr;
+  out->ke0 = c->k_exp.s[0]; out->ke1 = c->k_exp.s[1]; out->ke2 = c->k_exp.s[2];
+  out->ve0 = c->v_exp.s[0]; out->ve1 = c->v_exp.s[1]; out->ve2 = c->v_exp.s[2];
+  out->table = c->table; out->table_stride = c->table_stride;
+  out->table_len = (int)c->table_len; out->P = (int)c->pages; out->S = (int)c->page_size;
+  return 0;
+}
+
+// A dense operand: float32, bf16 or f16.
+int check_dense(const tension_buf* b, const char* what, int unit) {
+  TRY(check_buf(b, what, true, unit));
+  if (b->dtype == TENSION_F64) return fail(TENSION_ERR_UNSUPPORTED, "%s: the paged cache has no float64 form", what);
+  return 0;
+}
+
+int paged_rows(bool append, const tension_paged* cache, const tension_buf* k, const tension_buf* v,
+               const int32_t* start, const int32_t* counts, int64_t N, int64_t T, int64_t Hk, int64_t D,
+               tension_stream_t stream) {
+  const char* what = append ? "tension_paged_append" : "tension_paged_read";
+  if (N < 0 || T < 0 || Hk < 0 || D < 1 || D > 0xffff || T > 0x3fffffff || N > 0x3fffffff || Hk > 0xffff ||
+      mul_cap(mul_cap(N, T, (int64_t)1 << 40), Hk, (int64_t)1 << 40) < 0)
+    return fail(TENSION_ERR_ARG, "%s: bad sizes N=%lld T=%lld Hk=%lld D=%lld", what, (long long)N, (long long)T,
+                (long long)Hk, (long long)D);
+  if (N * T * Hk == 0) return ok();
+  PagedRowsParams p;
+  memset(&p, 0, sizeof p);
+  TRY(check_paged(cache, &p.c));
+  TRY(check_dense(k, "k", 3));
+  TRY(check_dense(v, "v", 3));
+  if (!start) return fail(TENSION_ERR_ARG, "start is required");
+  auto mix = [&](const tension_buf* x, const tension_buf& pages) {
+    return !append || pages.dtype == TENSION_E4M3 || pages.dtype == x->dtype ||
+           (x->dtype == TENSION_F32 && pages.dtype != TENSION_F32);
+  };
+  if (!mix(k, cache->k) || !mix(v, cache->v))
+    return fail(TENSION_ERR_ARG, "%s: tokens of another 16-bit type than their pages, or 16-bit tokens for float32 pages",
+                what);
+  p.kd = make_buf(k); p.vd = make_buf(v);
+  p.start = start; p.counts = counts;
+  p.N = (int)N; p.T = (int)T; p.Hk = (int)Hk; p.D = (int)D;
+  hipError_t e = hipSuccess;
+  launch_paged_rows(append, p, hs(stream), &e);
+  return launched(e, what);
+}
+
+// Sizes of a decode call; the bound of the lengths that shapes the launch.
+int paged_decode_sizes(int64_t N, int64_t H, int64_t Hk, int64_t D, int64_t W, int64_t max_len, int64_t table_len,
+                       int64_t page_size, int64_t* bound) {
+  if (N < 0 || H < 0 || Hk < 0 || D < 1 || D > 256 || W < 0 || W > 0x3fffffff || max_len < 0 || table_len < 0 ||
+      table_len > 0x7fffffff || page_size < 1 || page_size > 0x3fffffff || mul_cap(N, H, 0x7fffff) < 0 ||
+      (H > 0 && (Hk < 1 || H % Hk)))
+    return fail(TENSION_ERR_ARG,
+                "paged decode: bad sizes N=%lld H=%lld Hk=%lld D=%lld W=%lld max_len=%lld table_len=%lld page_size=%lld",
+                (long long)N, (long long)H, (long long)Hk, (long long)D, (long long)W, (long long)max_len,
+                (long long)table_len, (long long)page_size);
+  int64_t cap = mul_cap(table_len, page_size, 0x7fffffff);
+  if (cap < 0) cap = 0x7fffffff;
+  *bound = max_len > 0 && max_len < cap ? max_len : cap;
+  return 0;
+}
+
+}  // namespace
+
+int tension_paged_append(const tension_paged* cache, const tension_buf* k_new, const tension_buf* v_new,
+                         const int32_t* start, const int32_t* counts, int64_t N, int64_t T, int64_t Hk, int64_t D,
+                         tension_stream_t stream) {
+  return paged_rows(true, cache, k_new, v_new, start, counts, N, T, Hk, D, stream);
+}
+
+int tension_paged_read(const tension_paged* cache, const tension_buf* k_out, const tension_buf* v_out,
+                       const int32_t* start, const int32_t* counts, int64_t N, int64_t T, int64_t Hk, int64_t D,
+                       tension_stream_t stream) {
+  return paged_rows(false, cache, k_out, v_out, start, counts, N, T, Hk, D, stream);
+}
+
+int64_t tension_paged_decode_workspace(int64_t N, int64_t H, int64_t Hk, int64_t D, int64_t W, int64_t max_len,
+                                       int64_t table_len, int64_t page_size) {
+  int64_t bound = 0;
+  if (paged_decode_sizes(N, H, Hk, D, W, max_len, table_len, page_size, &bound)) return -1;
+  int splits = 1, chunk = 0;
+  if (N * H > 0) paged_decode_split(N, H, Hk, D, W, bound, &splits, &chunk);
+  return splits > 1 ? N * H * splits * (D + 1) * (int64_t)sizeof(float) : 0;
+}
+
+int tension_paged_decode(const tension_paged* cache, const tension_buf* q, const tension_buf* out,
+                         const int32_t* lengths, void* workspace, int64_t N, int64_t H, int64_t Hk, int64_t D,
+                         int64_t W, int64_t max_len, double scale, int32_t flags, tension_stream_t stream) {
+  int64_t bound = 0;
+  TRY(paged_decode_sizes(N, H, Hk, D, W, max_len, cache ? cache->table_len : 0, cache ? cache->page_size : 1, &bound));
+  if (!(std::isfinite(scale) && scale != 0.0)) return fail(TENSION_ERR_ARG, "scale must be finite and non-zero");
+  if (N * H == 0) return ok();
+  PagedDecodeParams p;
+  memset(&p, 0, sizeof p);
+  TRY(check_paged(cache, &p.c));
+  TRY(check_dense(q, "q", 2));
+  TRY(check_dense(out, "out", 2));
+  if (q->dtype != out->dtype) return fail(TENSION_ERR_ARG, "paged decode: q and out must have one dtype");
+  if (!lengths) return fail(TENSION_ERR_ARG, "lengths is required");
+  if ((flags & TENSION_NORM_MASS) && (flags & TENSION_NORM_COUNT))
+    return fail(TENSION_ERR_ARG, "paged decode: TENSION_NORM_MASS and TENSION_NORM_COUNT are exclusive");
+  p.q = make_buf(q); p.out = make_buf(out); p.lengths = lengths; p.ws = (float*)workspace;
+  p.N = (int)N; p.H = (int)H; p.Hk = (int)Hk; p.D = (int)D; p.W = (int)W;
+  p.scale = (float)scale; p.inv_scale = (float)(1.0 / scale); p.flags = flags;
+  paged_decode_split(N, H, Hk, D, W, bound, &p.splits, &p.chunk);
+  if (p.splits > 1 && !workspace) return fail(TENSION_ERR_ARG, "paged decode: workspace is required");
+  hipError_t e = hipSuccess;
+  launch_paged_decode(p, hs(stream), &e);
+  return launched(e, "tension_paged_decode");
+}
+
 int tension_bias_table_insert(const uint64_t* keys_in, const double* vals_in, int64_t n, uint64_t* table_keys,
                               double* table_vals, int32_t log2cap, tension_stream_t stream) {
   if (log2cap < 1 || log2cap > 40) return fail(TENSION_ERR_ARG, "bias table: log2cap=%d outside [1, 40]", log2cap);

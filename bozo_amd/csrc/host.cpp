@@ -1,6 +1,6 @@
 // The eager call path in native code: output and workspace allocation, the
 // tension_buf descriptors, the library call and the autograd nodes of the
-// window op, the global block, RoPE and the decode step.
+// window op, the global block, RoPE, the decode step and the paged cache.
 //
 // A forward + backward through Python autograd Functions and ctypes cost the
 // host about 170 us, most of it in the engine's device thread (the GIL taken
@@ -325,6 +325,128 @@ OptTensor decode_step(const Tensor& q, const Tensor& kn, const Tensor& vn, const
   return out;
 }
 
+// -------------------------------------------------------------- paged cache
+
+// The four tensors of a cache, its table, and whether they fit each other.
+struct Paged {
+  tension_paged c{};
+  bool fits = false;
+  Tensor table;
+  Paged(const Tensor& k, const Tensor& v, const OptTensor& ke, const OptTensor& ve, const Tensor& table_, int64_t N,
+        bool written) {
+    if (!k.is_cuda() || k.dim() != 4 || v.sizes() != k.sizes() || v.device() != k.device() || k.size(0) < 1 ||
+        k.size(2) < 1 || table_.scalar_type() != at::kInt || table_.dim() != 2 || table_.size(0) != N ||
+        table_.device() != k.device())
+      return;
+    if (!one(k, ke, written, &c.k, &c.k_exp) || !one(v, ve, written, &c.v, &c.v_exp)) return;
+    table = table_.stride(1) == 1 || table_.size(1) <= 1 ? table_ : table_.contiguous();
+    c.table = table.const_data_ptr<int32_t>();
+    c.table_stride = table.stride(0);
+    c.table_len = table.size(1);
+    c.pages = k.size(0);
+    c.page_size = k.size(2);
+    // an empty table has no memory; no entry of it is read
+    if (!c.table) c.table = (const int32_t*)k.const_data_ptr();
+    fits = true;
+  }
+
+ private:
+  static bool one(const Tensor& t, const OptTensor& e_, bool written, tension_buf* b, tension_buf* eb) {
+    const bool quantised = t.scalar_type() == at::kFloat8_e4m3fn;
+    const int code = quantised ? (int)TENSION_E4M3 : t.scalar_type() == at::kDouble ? -1 : dtype_code(t);
+    if (code < 0 || t.stride(3) != 1 || quantised != (e_.has_value() && e_->defined())) return false;
+    b->ptr = written ? t.mutable_data_ptr() : const_cast<void*>(t.const_data_ptr());
+    b->dtype = code;
+    for (int i = 0; i < 4; ++i) b->s[i] = t.stride(i);
+    if (!quantised) return true;
+    const Tensor& e = *e_;
+    if (e.scalar_type() != at::kByte || e.dim() != 3 || e.sizes() != t.sizes().slice(0, 3) || e.device() != t.device())
+      return false;
+    eb->ptr = written ? e.mutable_data_ptr() : const_cast<void*>(e.const_data_ptr());
+    eb->dtype = TENSION_U8;
+    for (int i = 0; i < 3; ++i) eb->s[i] = e.stride(i);
+    return true;
+  }
+};
+
+bool dense_ok(at::ScalarType t) { return t == at::kFloat || t == at::kBFloat16 || t == at::kHalf; }
+
+// int32 [N] counters of a call.
+bool counter_ok(const Tensor& t, int64_t N, const Tensor& like) {
+  return !t.defined() || (t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == N && t.device() == like.device());
+}
+const int32_t* counter_ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr<int32_t>() : nullptr; }
+
+// False when an operand does not fit the others (the caller then says which),
+// likewise below.
+bool paged_append(const Tensor& k, const Tensor& v, const OptTensor& ke, const OptTensor& ve, const Tensor& kn,
+                  const Tensor& vn, const Tensor& table, const Tensor& start, const OptTensor& counts_) {
+  if (kn.dim() != 4 || vn.sizes() != kn.sizes() || !dense_ok(kn.scalar_type()) || !dense_ok(vn.scalar_type()) ||
+      kn.device() != k.device() || vn.device() != k.device() || k.dim() != 4 || kn.size(2) != k.size(1) ||
+      kn.size(3) != k.size(3))
+    return false;
+  const int64_t N = kn.size(0);
+  const Tensor counts = opt(counts_);
+  if (!counter_ok(start, N, k) || !counter_ok(counts, N, k)) return false;
+  for (const auto& [x, pages] : {std::pair(kn, k), std::pair(vn, v)}) {
+    const at::ScalarType a = x.scalar_type(), b = pages.scalar_type();
+    if (b != at::kFloat8_e4m3fn && a != b && !(a == at::kFloat && dense_ok(b))) return false;
+  }
+  if (!k.is_cuda()) return false;
+  const c10::DeviceGuard guard(k.device());
+  const Paged c(k, v, ke, ve, table, N, true);
+  if (!c.fits) return false;
+  if (kn.numel() == 0) return true;
+  const Tensor knr = rows(kn), vnr = rows(vn), st = start.contiguous(), ct = counts.defined() ? counts.contiguous() : counts;
+  const Buf bk(knr), bv(vnr);
+  check(tension_paged_append(&c.c, bk.get(), bv.get(), counter_ptr(st), counter_ptr(ct), N, kn.size(1), kn.size(2),
+                             kn.size(3), stream_of(k)),
+        "tension_paged_append");
+  return true;
+}
+
+std::optional<std::tuple<Tensor, Tensor>> paged_read(const Tensor& k, const Tensor& v, const OptTensor& ke,
+                                                     const OptTensor& ve, const Tensor& table, const Tensor& start,
+                                                     int64_t T, at::ScalarType kdt, at::ScalarType vdt,
+                                                     const OptTensor& counts_) {
+  if (T < 0 || !dense_ok(kdt) || !dense_ok(vdt) || start.dim() != 1 || k.dim() != 4 || !k.is_cuda()) return std::nullopt;
+  const int64_t N = start.size(0), Hk = k.size(1), D = k.size(3);
+  const Tensor counts = opt(counts_);
+  if (!counter_ok(start, N, k) || !counter_ok(counts, N, k)) return std::nullopt;
+  const c10::DeviceGuard guard(k.device());
+  const Paged c(k, v, ke, ve, table, N, false);
+  if (!c.fits) return std::nullopt;
+  Tensor ko = empty({N, T, Hk, D}, kdt, k), vo = empty({N, T, Hk, D}, vdt, k);
+  if (ko.numel() == 0) return std::make_tuple(ko, vo);
+  const Tensor st = start.contiguous(), ct = counts.defined() ? counts.contiguous() : counts;
+  const Buf bk = written(ko), bv = written(vo);
+  check(tension_paged_read(&c.c, bk.get(), bv.get(), counter_ptr(st), counter_ptr(ct), N, T, Hk, D, stream_of(k)),
+        "tension_paged_read");
+  return std::make_tuple(ko, vo);
+}
+
+OptTensor paged_decode(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& ke, const OptTensor& ve,
+                       const Tensor& table, const Tensor& lengths, double scale, int64_t W, int64_t max_len,
+                       int64_t flags) {
+  if (q.dim() != 3 || !q.is_cuda() || !dense_ok(q.scalar_type()) || k.dim() != 4 || q.device() != k.device() ||
+      q.size(2) != k.size(3) || W < 0 || max_len < 0)
+    return std::nullopt;
+  const int64_t N = q.size(0), H = q.size(1), D = q.size(2), Hk = k.size(1);
+  if (!counter_ok(lengths, N, q) || Hk < 1 || H % Hk) return std::nullopt;
+  const c10::DeviceGuard guard(q.device());
+  const Paged c(k, v, ke, ve, table, N, false);
+  if (!c.fits) return std::nullopt;
+  Tensor out = empty(q.sizes(), q);
+  if (q.numel() == 0) return out;
+  const Tensor qr = rows(q), len = lengths.contiguous();
+  const Tensor ws = workspace(tension_paged_decode_workspace(N, H, Hk, D, W, max_len, c.c.table_len, c.c.page_size), q);
+  const Buf bq(qr), bo = written(out);
+  check(tension_paged_decode(&c.c, bq.get(), bo.get(), counter_ptr(len), ptr(ws), N, H, Hk, D, W, max_len, scale,
+                             (int32_t)flags, stream_of(q)),
+        "tension_paged_decode");
+  return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_host, m) {
@@ -376,4 +498,12 @@ PYBIND11_MODULE(_host, m) {
     return RopeFn::apply(rows(x), cos.contiguous(), sin.contiguous(), pos_offset, dt);
   });
   m.def("decode_step", &decode_step, release());
+  m.def("paged_append", &paged_append, release());
+  m.def("paged_read", [](const Tensor& k, const Tensor& v, const OptTensor& ke, const OptTensor& ve, const Tensor& table,
+                         const Tensor& start, int64_t T, py::object kdt, py::object vdt, const OptTensor& counts) {
+    const at::ScalarType a = torch::python::detail::py_object_to_dtype(kdt), b = torch::python::detail::py_object_to_dtype(vdt);
+    py::gil_scoped_release r;
+    return paged_read(k, v, ke, ve, table, start, T, a, b, counts);
+  });
+  m.def("paged_decode", &paged_decode, release());
 }

@@ -74,6 +74,41 @@ struct AuxLossParams {
   int L, B, T, H, W;
 };
 
+// paged cache (paged.hip, paged_decode.hip)
+struct PagedCache {
+  Buf k, v;                        // [P, Hk, S, D]
+  const uint8_t *ke, *ve;          // [P, Hk, S], null unless e4m3
+  int64_t ke0, ke1, ke2, ve0, ve1, ve2;
+  const int32_t* table;            // [N, table_len]
+  int64_t table_stride;
+  int table_len, P, S;
+};
+
+struct PagedRowsParams {  // append (dense -> pages) and read (pages -> dense)
+  PagedCache c;
+  Buf kd, vd;             // [N, T, Hk, D]
+  const int32_t* start;
+  const int32_t* counts;  // nullable
+  int N, T, Hk, D;
+};
+
+struct PagedDecodeParams {
+  PagedCache c;
+  Buf q, out;  // [N, H, D]
+  const int32_t* lengths;
+  float* ws;   // [N * H, splits, D + 1] partial sums and masses, null when splits == 1
+  int N, H, Hk, D, W;
+  int splits, chunk;  // split i: keys from lo + i * chunk, the last one to the end
+  float scale, inv_scale;
+  int flags;
+};
+
+// Keys per split and splits of a decode call (one rule for the workspace
+// query and the launch).
+void paged_decode_split(int64_t N, int64_t H, int64_t Hk, int64_t D, int64_t W, int64_t max_len, int* splits, int* chunk);
+int launch_paged_rows(bool append, const PagedRowsParams& p, hipStream_t st, hipError_t* err);
+int launch_paged_decode(const PagedDecodeParams& p, hipStream_t st, hipError_t* err);
+
 // phase: 0 forward, 1 dQ, 2 dK/dV.  Return 0 when launched (HIP status in
 // *err), -1 when no kernel exists for the request, kGridTooLarge when the
 // grid would exceed 2^31 - 1 workgroups (band.h).

@@ -41,7 +41,10 @@ enum {
   TENSION_F32 = 0,
   TENSION_BF16 = 1,
   TENSION_F16 = 2,
-  TENSION_F64 = 3
+  TENSION_F64 = 3,
+  /* pages of a paged cache only */
+  TENSION_E4M3 = 4, /* 8-bit float, 4 exponent and 3 mantissa bits, no infinity */
+  TENSION_U8 = 5    /* exponent bytes */
 };
 
 /* status codes */
@@ -344,6 +347,75 @@ int tension_bias_build(const int32_t* content_ids, int64_t B, int64_t T,
                        const double* table_vals, int32_t log2cap,
                        double alpha, const tension_buf* bias, double* stats,
                        tension_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Paged K/V cache: tokens of sequences of different lengths in pages of S
+ * tokens from one pool (no counterpart in the reference, whose generation
+ * keeps no cache, model.py:736-739).
+ *   k, v: [P,Hk,S,D] pages (s[0..3], s[3] == 1; P = pages, S = page_size),
+ *     float32, bf16, f16 or e4m3, each its own type.  A page may lie beyond
+ *     2^32 elements from the first.
+ *   k_exp, v_exp: [P,Hk,S] exponent bytes (s[0..2], TENSION_U8) of an e4m3
+ *     buffer, ptr NULL otherwise: a row's value is code * 2^(byte - 127).
+ *   table: device int32 [N,table_len], row stride table_stride: page
+ *     table[n][pos / S] holds position pos of sequence n at row pos % S.
+ *     An entry outside [0, P) is no page: its tokens are not written, read
+ *     back as zeros, and attended to by nothing.
+ * ------------------------------------------------------------------------- */
+typedef struct tension_paged {
+  tension_buf k, v, k_exp, v_exp;
+  const int32_t* table;
+  int64_t table_stride, table_len, pages, page_size;
+} tension_paged;
+
+/* Writes tokens k_new, v_new [N,T,Hk,D] (float32, bf16 or f16) at positions
+ * start[n] .. start[n] + counts[n] - 1 (device int32 [N]; counts NULL = T,
+ * clamped to [0, T]); positions below 0 or past the table are left out.
+ *   Pages of the source's type take the values as they are, bf16 or f16
+ * pages of float32 tokens the nearest ones (other mixes are refused), e4m3
+ * pages per row the smallest power of two 2^e, e >= -126, with max |x| <=
+ * 448 * 2^e over the row's finite values, and x / 2^e rounded to nearest
+ * even; infinities become NaN.  Two tokens of one call in one place leave one of them. */
+int tension_paged_append(const tension_paged* cache, const tension_buf* k_new,
+                         const tension_buf* v_new, const int32_t* start,
+                         const int32_t* counts, int64_t N, int64_t T,
+                         int64_t Hk, int64_t D, tension_stream_t stream);
+
+/* Reads positions start[n] + t back into k_out, v_out [N,T,Hk,D] (float32,
+ * bf16 or f16, each its own type; every element written): zeros for t >=
+ * counts[n], positions below 0 or past the table, and entries that are no
+ * page. */
+int tension_paged_read(const tension_paged* cache, const tension_buf* k_out,
+                       const tension_buf* v_out, const int32_t* start,
+                       const int32_t* counts, int64_t N, int64_t T, int64_t Hk,
+                       int64_t D, tension_stream_t stream);
+
+/* One new token per sequence over its cached tokens (the step of
+ * tension_decode_step on pages; the new token is in the cache already).
+ *   q, out: [N,H,D] (s[0..2]), float32, bf16 or f16, alike; H a multiple of
+ *   Hk, query head h reads key head h / (H / Hk).  D <= 256.
+ *   lengths: device int32 [N], cached tokens of each sequence, the newest at
+ *   position lengths[n] - 1 (clamped to [0, table_len * S]).
+ *   Keys lo <= s < hi: hi = lengths[n] with TENSION_DECODE_SELF, else
+ *   lengths[n] - 1; lo = max(0, lengths[n] - 1 - W), or 0 with W == 0.
+ *   out = sum tau v, tau = sigmoid(q . k / scale), divided by max(sum tau,
+ *   1e-6) with TENSION_NORM_MASS, by max(hi - lo, 1) with
+ *   TENSION_NORM_COUNT; zeros where there is no key.  Rows of keys outside
+ *   [lo, hi) are not read.
+ *   max_len: a bound of the lengths that the host knows (0: none); it only
+ *   shapes the launch, a longer sequence is attended to in full.
+ *   workspace: tension_paged_decode_workspace() bytes for the same sizes
+ *   (NULL if that is 0; -1 for sizes the entry point rejects).  The keys
+ *   of a sequence are split over workgroups where there are few rows; the
+ *   partial sums meet there and are added in a fixed order. */
+int64_t tension_paged_decode_workspace(int64_t N, int64_t H, int64_t Hk,
+                                       int64_t D, int64_t W, int64_t max_len,
+                                       int64_t table_len, int64_t page_size);
+int tension_paged_decode(const tension_paged* cache, const tension_buf* q,
+                         const tension_buf* out, const int32_t* lengths,
+                         void* workspace, int64_t N, int64_t H, int64_t Hk,
+                         int64_t D, int64_t W, int64_t max_len, double scale,
+                         int32_t flags, tension_stream_t stream);
 
 /* Message for the last non-OK return on the calling thread ("" if none). */
 const char* tension_last_error(void);
