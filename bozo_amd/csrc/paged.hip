@@ -8,6 +8,8 @@
 // of two scales exactly, so the one rounding of a value is that of its code
 // (e4m3, half a step: 2^-4 relative), and a float scale would buy nothing: an
 // e4m3 code's relative step does not depend on where in its range it lies.
+#include <type_traits>
+
 #include "kernels.h"
 
 namespace tension {
@@ -118,9 +120,273 @@ __global__ void __launch_bounds__(kThreads) paged_rows_any(PagedRowsParams p) {
     any_row<APPEND>(p, r, threadIdx.x & 63);
 }
 
+// ------------------------------------------------------------------ whole pieces of 8 values
+
+// n / d for n < 2^31 as a multiplication (rounded-up reciprocal).
+struct FastDiv {
+  unsigned m;
+  int s;
+};
+__device__ __forceinline__ int fdiv(int n, FastDiv d) { return (int)((__umulhi((unsigned)n, d.m) + (unsigned)n) >> d.s); }
+
+FastDiv fast_div(int64_t d) {
+  int s = 0;
+  while (((int64_t)1 << s) < d) ++s;
+  return {(unsigned)(((uint64_t)1 << 32) * (((uint64_t)1 << s) - d) / d + 1), s};
+}
+
+struct VecGeometry {
+  FastDiv heads, tiles, page;
+  int ntile, lg_tile;  // tiles of 2^lg_tile tokens of one sequence
+  int units;           // N * ntile * Hk * 2^lg_tile rows
+};
+
+template <int CTRL>
+__device__ __forceinline__ unsigned dpp_umax(unsigned x) {
+  const unsigned o = (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xF, 0xF, true);
+  return o > x ? o : x;
+}
+
+// Largest over an aligned group of LPR lanes.
+template <int LPR>
+__device__ __forceinline__ unsigned group_umax(unsigned x) {
+  if constexpr (LPR >= 2) x = dpp_umax<0xB1>(x);    // lane ^ 1
+  if constexpr (LPR >= 4) x = dpp_umax<0x4E>(x);    // lane ^ 2
+  if constexpr (LPR >= 8) x = dpp_umax<0x141>(x);   // mirrored halves of 8
+  if constexpr (LPR >= 16) x = dpp_umax<0x140>(x);  // mirrored rows of 16
+  if constexpr (LPR >= 32) {
+    const unsigned o = (unsigned)__shfl_xor((int)x, 16);
+    x = o > x ? o : x;
+  }
+  return x;
+}
+
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+
+// Eight dense values as they are loaded, and as floats.
+template <bool F32>
+struct Eight {
+  u32x4 a[F32 ? 2 : 1];
+  __device__ __forceinline__ void load(const Buf& b, int64_t off) {
+    const u32x4* s = (const u32x4*)((const char*)b.p + off * (F32 ? 4 : 2));
+    a[0] = s[0];
+    if constexpr (F32) a[1] = s[1];
+  }
+  __device__ __forceinline__ void store(const Buf& b, int64_t off) const {
+    u32x4* s = (u32x4*)((char*)const_cast<void*>(b.p) + off * (F32 ? 4 : 2));
+    s[0] = a[0];
+    if constexpr (F32) s[1] = a[1];
+  }
+  __device__ __forceinline__ void floats(bool half, float* x) const {
+    if constexpr (F32) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const unsigned w = a[i / 4][i % 4];  // a copy: bit_cast of a vector's element takes element 0
+        x[i] = __builtin_bit_cast(float, w);
+      }
+    } else if (half) {
+      const f16x8 h = __builtin_bit_cast(f16x8, a[0]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = (float)h[i];
+    } else {
+      const bf16x8 h = __builtin_bit_cast(bf16x8, a[0]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = (float)h[i];
+    }
+  }
+  __device__ __forceinline__ void set(bool half, const float* x) {
+    if constexpr (F32) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a[i / 4][i % 4] = __builtin_bit_cast(unsigned, x[i]);
+    } else if (half) {
+      f16x8 h;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[i] = (f16)x[i];
+      a[0] = __builtin_bit_cast(u32x4, h);
+    } else {
+      bf16x8 h;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[i] = (bf16)x[i];
+      a[0] = __builtin_bit_cast(u32x4, h);
+    }
+  }
+};
+
+// LPR lanes to a row, eight values to a lane, R rows to a thread (their loads
+// ahead of the first use).  A workgroup's consecutive rows are tokens of one
+// head: their places in a page lie together, and in the dense tensor each is a
+// piece of D values of its token.
+template <bool APPEND, int LPR, int R, bool F32>
+__device__ __forceinline__ void vec_rows(const PagedRowsParams& p, const VecGeometry& g, bool isv) {
+  constexpr int kRows = kThreads / LPR;
+  const Buf& pg = isv ? p.c.v : p.c.k;
+  const Buf& de = isv ? p.vd : p.kd;
+  uint8_t* ex = const_cast<uint8_t*>(isv ? p.c.ve : p.c.ke);
+  const int64_t e0 = isv ? p.c.ve0 : p.c.ke0, e1 = isv ? p.c.ve1 : p.c.ke1, e2 = isv ? p.c.ve2 : p.c.ke2;
+  const int ch = threadIdx.x % LPR * 8;
+  int64_t doff[R], poff[R], eoff[R];
+  bool live[R], in[R];
+  Eight<F32> x[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int u = (blockIdx.x * R + r) * kRows + threadIdx.x / LPR;
+    const int y = u >> g.lg_tile, z = fdiv(y, g.heads), h = y - z * p.Hk;
+    const int n = fdiv(z, g.tiles), t = ((z - n * g.ntile) << g.lg_tile) + (u & ((1 << g.lg_tile) - 1));
+    in[r] = u < g.units && t < p.T;
+    doff[r] = n * de.s0 + t * de.s1 + h * de.s2 + ch;
+    live[r] = false;
+    int pos = 0;
+    if (in[r] && token_pos(p, n, t, &pos)) {
+      const int slot = fdiv(pos, g.page), row = pos - slot * p.c.S;
+      if (APPEND) x[r].load(de, doff[r]);
+      if (slot < p.c.table_len) {
+        const int id = p.c.table[(int64_t)n * p.c.table_stride + slot];
+        live[r] = id >= 0 && id < p.c.P;
+        poff[r] = id * pg.s0 + h * pg.s1 + row * pg.s2 + ch;
+        eoff[r] = id * e0 + h * e1 + row * e2;
+      }
+    }
+  }
+  const bool half = de.dt == TENSION_F16, quantised = pg.dt == TENSION_E4M3;
+  if constexpr (APPEND) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (!live[r]) continue;  // a row's lanes agree
+      if (!quantised) {
+        if (pg.dt == de.dt) {
+          x[r].store(pg, poff[r]);
+        } else {  // float32 tokens, 16-bit pages
+          float f[8];
+          x[r].floats(half, f);
+          Eight<false> y;
+          y.set(pg.dt == TENSION_F16, f);
+          y.store(pg, poff[r]);
+        }
+        continue;
+      }
+      float f[8];
+      x[r].floats(half, f);
+      unsigned top = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const unsigned b = finite_bits(f[i]);
+        top = b > top ? b : top;
+      }
+      const int b = exp_byte(group_umax<LPR>(top));
+      const float inv = pow2_of_byte(254 - b);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = to_code_range(f[i], inv);
+      *(u32x2*)((uint8_t*)pg.p + poff[r]) = u32x2{pack4(f[0], f[1], f[2], f[3]), pack4(f[4], f[5], f[6], f[7])};
+      if (ch == 0) ex[eoff[r]] = (uint8_t)b;
+    }
+  } else {
+    if (quantised) {
+      u32x2 c[R];
+      uint8_t b[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        c[r] = live[r] ? *(const u32x2*)((const uint8_t*)pg.p + poff[r]) : u32x2{0, 0};
+        b[r] = live[r] ? ex[eoff[r]] : 127;
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float f[8];
+        const float s = pow2_of_byte(b[r]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          f[4 * i] = __builtin_amdgcn_cvt_f32_fp8((int)c[r][i], 0) * s;
+          f[4 * i + 1] = __builtin_amdgcn_cvt_f32_fp8((int)c[r][i], 1) * s;
+          f[4 * i + 2] = __builtin_amdgcn_cvt_f32_fp8((int)c[r][i], 2) * s;
+          f[4 * i + 3] = __builtin_amdgcn_cvt_f32_fp8((int)c[r][i], 3) * s;
+        }
+        x[r].set(half, f);
+        if (in[r]) x[r].store(de, doff[r]);
+      }
+      return;
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (!in[r]) continue;
+      float f[8] = {};
+      if (!live[r]) {
+        x[r].set(half, f);
+      } else if (pg.dt == de.dt) {
+        x[r].load(pg, poff[r]);
+      } else if (pg.dt == TENSION_F32) {
+        Eight<true> y;
+        y.load(pg, poff[r]);
+        y.floats(false, f);
+        x[r].set(half, f);
+      } else {
+        Eight<false> y;
+        y.load(pg, poff[r]);
+        y.floats(pg.dt == TENSION_F16, f);
+        x[r].set(half, f);
+      }
+      x[r].store(de, doff[r]);
+    }
+  }
+}
+
+template <bool APPEND, int LPR, int R>
+__global__ void __launch_bounds__(kThreads) paged_rows_vec(PagedRowsParams p, VecGeometry g) {
+  const bool isv = blockIdx.y != 0;
+  if ((isv ? p.vd.dt : p.kd.dt) == TENSION_F32)
+    vec_rows<APPEND, LPR, R, true>(p, g, isv);
+  else
+    vec_rows<APPEND, LPR, R, false>(p, g, isv);
+}
+
+// Pieces of 8 values of a row are whole 16-byte (8-byte: e4m3) pieces of memory.
+bool vec_aligned(const Buf& b) {
+  const int64_t bytes = b.dt == TENSION_E4M3 ? 1 : b.dt == TENSION_F32 ? 4 : 2, to = b.dt == TENSION_E4M3 ? 8 : 16;
+  return (uintptr_t)b.p % to == 0 && b.s0 * bytes % to == 0 && b.s1 * bytes % to == 0 && b.s2 * bytes % to == 0;
+}
+
+template <bool APPEND, int R>
+bool launch_vec(const PagedRowsParams& p, const VecGeometry& g, hipStream_t st) {
+  auto go = [&](auto lanes) {
+    constexpr int LPR = decltype(lanes)::value;
+    const int per = kThreads / LPR * R;
+    paged_rows_vec<APPEND, LPR, R><<<dim3((unsigned)((g.units + per - 1) / per), 2), kThreads, 0, st>>>(p, g);
+    return true;
+  };
+  switch (p.D) {
+    case 32: return go(std::integral_constant<int, 4>{});
+    case 64: return go(std::integral_constant<int, 8>{});
+    case 128: return go(std::integral_constant<int, 16>{});
+    case 256: return go(std::integral_constant<int, 32>{});
+    default: return false;
+  }
+}
+
+// Head dims 32 to 256 (powers of two) with aligned rows.
+bool try_vec(bool append, const PagedRowsParams& p, hipStream_t st) {
+  if (!vec_aligned(p.kd) || !vec_aligned(p.vd) || !vec_aligned(p.c.k) || !vec_aligned(p.c.v)) return false;
+  VecGeometry g;
+  g.lg_tile = 0;
+  while (g.lg_tile < 5 && (1 << g.lg_tile) < p.T) ++g.lg_tile;
+  g.ntile = (int)(((int64_t)p.T + (1 << g.lg_tile) - 1) >> g.lg_tile);
+  const int64_t units = mul_cap(mul_cap((int64_t)p.N * g.ntile, p.Hk, 1 << 30), (int64_t)1 << g.lg_tile, 1 << 30);
+  if (units < 0) return false;
+  g.units = (int)units;
+  g.heads = fast_div(p.Hk);
+  g.tiles = fast_div(g.ntile);
+  g.page = fast_div(p.c.S);
+  // several rows to a thread once the grid fills the card many times over
+  const bool many = units * (p.D / 8) >= (int64_t)kThreads * device_cus() * 32;
+  if (append) return many ? launch_vec<true, 4>(p, g, st) : launch_vec<true, 1>(p, g, st);
+  return many ? launch_vec<false, 4>(p, g, st) : launch_vec<false, 1>(p, g, st);
+}
+
 }  // namespace
 
 int launch_paged_rows(bool append, const PagedRowsParams& p, hipStream_t st, hipError_t* err) {
+  if (try_vec(append, p, st)) {
+    *err = hipGetLastError();
+    return 0;
+  }
   const int64_t rows = (int64_t)p.N * p.Hk * p.T;
   int64_t grid = (rows + kThreads / 64 - 1) / (kThreads / 64);
   grid = grid < kMaxGrid ? grid : kMaxGrid;
