@@ -1,0 +1,71 @@
+// Device helpers of the paged cache: division by the page size, exponent bytes,
+// the keys of a sequence, how they are split over workgroups, and where the
+// sums of a split go.
+#pragma once
+
+#include "kernels.h"
+
+namespace tension {
+
+// n / d for n < 2^31 as a multiplication (rounded-up reciprocal).
+struct FastDiv {
+  unsigned m;
+  int s;
+};
+__device__ __forceinline__ int fdiv(int n, FastDiv d) { return (int)((__umulhi((unsigned)n, d.m) + (unsigned)n) >> d.s); }
+
+inline FastDiv fast_div(int64_t d) {
+  int s = 0;
+  while (((int64_t)1 << s) < d) ++s;
+  return {(unsigned)(((uint64_t)1 << 32) * (((uint64_t)1 << s) - d) / d + 1), s};
+}
+
+struct KeyRange {
+  int lo, hi;
+};
+
+// Keys of sequence n; the length is held to what the table can name.
+__device__ __forceinline__ KeyRange key_range(const PagedDecodeParams& p, int n) {
+  const int cap = (int)(p.c.table_len > 0x7fffffff / p.c.S ? 0x7fffffff : p.c.table_len * p.c.S);
+  int len = p.lengths[n];
+  len = len < 0 ? 0 : len > cap ? cap : len;
+  const int hi = (p.flags & TENSION_DECODE_SELF) ? len : len - 1;
+  const int lo = p.W > 0 && len - 1 > p.W ? len - 1 - p.W : 0;
+  return {lo, hi > lo ? hi : lo};
+}
+
+// Splits of a sequence that hold keys.
+__device__ __forceinline__ int used_splits(const PagedDecodeParams& p, KeyRange r) {
+  const int n = (int)(((int64_t)r.hi - r.lo + p.chunk - 1) / p.chunk);
+  return n < p.splits ? n : p.splits;
+}
+
+// Keys of split i (the last one takes what is left).
+__device__ __forceinline__ KeyRange split_range(const PagedDecodeParams& p, KeyRange r, int i) {
+  const int64_t a = r.lo + (int64_t)i * p.chunk;
+  const int64_t b = i == p.splits - 1 ? r.hi : a + p.chunk;
+  return {(int)(a < r.hi ? a : r.hi), (int)(b < r.hi ? b : r.hi)};
+}
+
+__device__ __forceinline__ float norm_factor(const PagedDecodeParams& p, float mass, KeyRange r) {
+  if (p.flags & TENSION_NORM_MASS) return 1.f / (mass > kMassEps ? mass : kMassEps);
+  if (p.flags & TENSION_NORM_COUNT) return 1.f / (float)(r.hi - r.lo > 1 ? r.hi - r.lo : 1);
+  return 1.f;
+}
+
+// Partial sums [N * H, splits, D], then the masses [N * H, splits].
+__device__ __forceinline__ float* split_sums(const PagedDecodeParams& p, int nh, int i) {
+  return p.ws + ((int64_t)nh * p.splits + i) * p.D;
+}
+__device__ __forceinline__ float* split_mass(const PagedDecodeParams& p, int nh, int i) {
+  return p.ws + (int64_t)p.N * p.H * p.splits * p.D + (int64_t)nh * p.splits + i;
+}
+
+// Scale of an exponent byte.
+__device__ __forceinline__ float pow2_of_byte(int b) { return __builtin_bit_cast(float, (unsigned)b << 23); }
+
+// Kernels for whole 16-byte pieces of a row.  False when the call has no such
+// form; the caller then runs the kernel for any.
+bool launch_paged_decode_rows(const PagedDecodeParams& p, hipStream_t st);
+
+}  // namespace tension

@@ -10,7 +10,7 @@
 // e4m3 code's relative step does not depend on where in its range it lies.
 #include <type_traits>
 
-#include "kernels.h"
+#include "paged.h"
 
 namespace tension {
 
@@ -24,7 +24,6 @@ __device__ __forceinline__ int exp_byte(unsigned amax_bits) {
   const int e = (int)(amax_bits >> 23) - 8 + ((amax_bits & 0x7fffff) > 0x600000 ? 1 : 0);
   return e < 1 ? 1 : e;
 }
-__device__ __forceinline__ float pow2_of_byte(int b) { return __builtin_bit_cast(float, (unsigned)b << 23); }
 
 // Magnitude bits of a finite value, 0 for infinities and NaN.
 __device__ __forceinline__ unsigned finite_bits(float x) {
@@ -121,19 +120,6 @@ __global__ void __launch_bounds__(kThreads) paged_rows_any(PagedRowsParams p) {
 }
 
 // ------------------------------------------------------------------ whole pieces of 8 values
-
-// n / d for n < 2^31 as a multiplication (rounded-up reciprocal).
-struct FastDiv {
-  unsigned m;
-  int s;
-};
-__device__ __forceinline__ int fdiv(int n, FastDiv d) { return (int)((__umulhi((unsigned)n, d.m) + (unsigned)n) >> d.s); }
-
-FastDiv fast_div(int64_t d) {
-  int s = 0;
-  while (((int64_t)1 << s) < d) ++s;
-  return {(unsigned)(((uint64_t)1 << 32) * (((uint64_t)1 << s) - d) / d + 1), s};
-}
 
 struct VecGeometry {
   FastDiv heads, tiles, page;

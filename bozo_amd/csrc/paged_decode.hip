@@ -4,46 +4,13 @@
 // so the sums of disjoint key ranges simply add up: the axis is split over
 // workgroups where there are few rows, and a second kernel adds the partial
 // sums in order of the splits.
-#include "kernels.h"
+#include "paged.h"
 
 namespace tension {
 
 namespace {
 
 constexpr int kThreads = 256;
-
-struct KeyRange {
-  int lo, hi;
-};
-
-// Keys of sequence n; the length is held to what the table can name.
-__device__ __forceinline__ KeyRange key_range(const PagedDecodeParams& p, int n) {
-  const int cap = (int)(p.c.table_len > 0x7fffffff / p.c.S ? 0x7fffffff : p.c.table_len * p.c.S);
-  int len = p.lengths[n];
-  len = len < 0 ? 0 : len > cap ? cap : len;
-  const int hi = (p.flags & TENSION_DECODE_SELF) ? len : len - 1;
-  const int lo = p.W > 0 && len - 1 > p.W ? len - 1 - p.W : 0;
-  return {lo, hi > lo ? hi : lo};
-}
-
-// Splits of a sequence that hold keys.
-__device__ __forceinline__ int used_splits(const PagedDecodeParams& p, KeyRange r) {
-  const int n = (int)(((int64_t)r.hi - r.lo + p.chunk - 1) / p.chunk);
-  return n < p.splits ? n : p.splits;
-}
-
-// Keys of split i (the last one takes what is left).
-__device__ __forceinline__ KeyRange split_range(const PagedDecodeParams& p, KeyRange r, int i) {
-  const int64_t a = r.lo + (int64_t)i * p.chunk;
-  const int64_t b = i == p.splits - 1 ? r.hi : a + p.chunk;
-  return {(int)(a < r.hi ? a : r.hi), (int)(b < r.hi ? b : r.hi)};
-}
-
-__device__ __forceinline__ float norm_factor(const PagedDecodeParams& p, float mass, KeyRange r) {
-  if (p.flags & TENSION_NORM_MASS) return 1.f / (mass > kMassEps ? mass : kMassEps);
-  if (p.flags & TENSION_NORM_COUNT) return 1.f / (float)(r.hi - r.lo > 1 ? r.hi - r.lo : 1);
-  return 1.f;
-}
 
 __device__ __forceinline__ float ld_page(const Buf& b, int64_t off) {
   return b.dt == TENSION_E4M3 ? __builtin_amdgcn_cvt_f32_fp8((int)((const uint8_t*)b.p)[off], 0) : ld<float>(b, off);
@@ -75,10 +42,10 @@ __global__ void __launch_bounds__(kThreads) paged_decode_any(PagedDecodeParams p
         const int64_t ko = page * p.c.k.s0 + hk * p.c.k.s1 + row * p.c.k.s2;
         float s = 0.f;
         for (int d = 0; d < p.D; ++d) s += qs[d] * ld_page(p.c.k, ko + d);
-        if (p.c.ke) s *= __builtin_bit_cast(float, (unsigned)p.c.ke[page * p.c.ke0 + hk * p.c.ke1 + row * p.c.ke2] << 23);
+        if (p.c.ke) s *= pow2_of_byte(p.c.ke[page * p.c.ke0 + hk * p.c.ke1 + row * p.c.ke2]);
         w = sigmoid_exact(s / p.scale);
         mass += w;
-        if (p.c.ve) w *= __builtin_bit_cast(float, (unsigned)p.c.ve[page * p.c.ve0 + hk * p.c.ve1 + row * p.c.ve2] << 23);
+        if (p.c.ve) w *= pow2_of_byte(p.c.ve[page * p.c.ve0 + hk * p.c.ve1 + row * p.c.ve2]);
         vo = page * p.c.v.s0 + hk * p.c.v.s1 + row * p.c.v.s2;
       }
     }
@@ -96,38 +63,71 @@ __global__ void __launch_bounds__(kThreads) paged_decode_any(PagedDecodeParams p
   __syncthreads();
   mass = red[0] + red[1] + red[2] + red[3];
   if (p.splits > 1) {
-    float* w = p.ws + ((int64_t)nh * p.splits + i) * (p.D + 1);
-    if (tid < p.D) w[tid] = acc;
-    if (tid == 0) w[p.D] = mass;
+    if (tid < p.D) split_sums(p, nh, i)[tid] = acc;
+    if (tid == 0) *split_mass(p, nh, i) = mass;
   } else if (tid < p.D) {
     st<float>(p.out, n * p.out.s0 + h * p.out.s1 + tid, acc * norm_factor(p, mass, all));
   }
 }
 
-// Partial sums of the splits of one (n, h), added in their order.
-__global__ void __launch_bounds__(kThreads) paged_decode_join(PagedDecodeParams p) {
-  const int nh = blockIdx.x, n = nh / p.H, h = nh % p.H;
+// Partial sums of the splits of one (n, h): GROUPS of DP threads take every
+// GROUPS-th split each, four loads under way at a time, and meet in LDS.  The
+// order of the sums is fixed.
+template <int DP, int GROUPS>
+__global__ void __launch_bounds__(DP* GROUPS) paged_decode_join(PagedDecodeParams p) {
+  __shared__ float red[GROUPS][DP], mred[DP * GROUPS / 64];
+  const int nh = blockIdx.x, n = nh / p.H, h = nh % p.H, tid = threadIdx.x, d = tid % DP, g = tid / DP;
   const KeyRange all = key_range(p, n);
   const int used = used_splits(p, all);
-  const float* w = p.ws + (int64_t)nh * p.splits * (p.D + 1);
-  float mass = 0.f;
-  for (int i = 0; i < used; ++i) mass += w[(int64_t)i * (p.D + 1) + p.D];
-  const float f = norm_factor(p, mass, all);
-  for (int d = threadIdx.x; d < p.D; d += kThreads) {
-    float acc = 0.f;
-    for (int i = 0; i < used; ++i) acc += w[(int64_t)i * (p.D + 1) + d];
-    st<float>(p.out, n * p.out.s0 + h * p.out.s1 + d, acc * f);
+  float m = 0.f, acc = 0.f;
+  const float* mass = split_mass(p, nh, 0);
+  for (int i = tid; i < used; i += DP * GROUPS) m += mass[i];
+  if (d < p.D) {
+    const float* w = split_sums(p, nh, 0) + d;
+    for (int i = g; i < used; i += 4 * GROUPS) {
+      float x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int s = i + j * GROUPS;
+        x[j] = w[(int64_t)(s < used ? s : i) * p.D];
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc += i + j * GROUPS < used ? x[j] : 0.f;
+    }
   }
+#pragma unroll
+  for (int k = 32; k; k >>= 1) m += __shfl_xor(m, k);
+  if ((tid & 63) == 0) mred[tid >> 6] = m;
+  red[g][d] = acc;
+  __syncthreads();
+  if (tid >= p.D) return;
+  m = 0.f;
+  acc = 0.f;
+#pragma unroll
+  for (int i = 0; i < DP * GROUPS / 64; ++i) m += mred[i];
+#pragma unroll
+  for (int i = 0; i < GROUPS; ++i) acc += red[i][tid];
+  st<float>(p.out, n * p.out.s0 + h * p.out.s1 + tid, acc * norm_factor(p, m, all));
+}
+
+template <int DP>
+void launch_join(const PagedDecodeParams& p, hipStream_t st) {
+  if (p.splits > 1024 / DP)
+    paged_decode_join<DP, 1024 / DP><<<(unsigned)(p.N * p.H), 1024, 0, st>>>(p);
+  else
+    paged_decode_join<DP, 256 / DP><<<(unsigned)(p.N * p.H), 256, 0, st>>>(p);
 }
 
 }  // namespace
 
-// About four workgroups per CU, splits of 256 keys at least.
+// About four workgroups per CU (all of them resident), splits of 128 keys at
+// least.
 void paged_decode_split(int64_t N, int64_t H, int64_t Hk, int64_t D, int64_t W, int64_t max_len, int* splits, int* chunk) {
+  constexpr int target = 1024, least = 128;
   const int64_t keys = W > 0 && W + 1 < max_len ? W + 1 : max_len;
-  const int64_t rows = N * H;
-  int64_t ns = (1024 + rows - 1) / (rows > 0 ? rows : 1);
-  const int64_t most = (keys + 255) / 256;
+  const int64_t rows = N * Hk;
+  int64_t ns = (target + rows / 2) / (rows > 0 ? rows : 1);
+  const int64_t most = keys / least;
   ns = ns > most ? most : ns;
   if (ns <= 1) {
     *splits = 1;
@@ -140,10 +140,13 @@ void paged_decode_split(int64_t N, int64_t H, int64_t Hk, int64_t D, int64_t W, 
 }
 
 int launch_paged_decode(const PagedDecodeParams& p, hipStream_t st, hipError_t* err) {
-  paged_decode_any<<<(unsigned)((int64_t)p.N * p.H * p.splits), kThreads, 0, st>>>(p);
+  if (!launch_paged_decode_rows(p, st))
+    paged_decode_any<<<(unsigned)((int64_t)p.N * p.H * p.splits), kThreads, 0, st>>>(p);
   *err = hipGetLastError();
   if (*err == hipSuccess && p.splits > 1) {
-    paged_decode_join<<<(unsigned)(p.N * p.H), kThreads, 0, st>>>(p);
+    if (p.D <= 64) launch_join<64>(p, st);
+    else if (p.D <= 128) launch_join<128>(p, st);
+    else launch_join<256>(p, st);
     *err = hipGetLastError();
   }
   return 0;

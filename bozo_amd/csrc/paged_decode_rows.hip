@@ -1,0 +1,40 @@
+// Which paged decode calls run on whole pieces of rows, and on how many waves.
+#include "paged.h"
+
+namespace tension {
+
+bool launch_paged_rows_bf16(const PagedDecodeParams&, int waves, hipStream_t);
+bool launch_paged_rows_f16(const PagedDecodeParams&, int waves, hipStream_t);
+bool launch_paged_rows_f32(const PagedDecodeParams&, int waves, hipStream_t);
+bool launch_paged_rows_mixed(const PagedDecodeParams&, int waves, hipStream_t);
+bool launch_paged_rows_e4m3(const PagedDecodeParams&, int waves, hipStream_t);
+
+namespace {
+
+// Pieces of 8 values (16 for e4m3 rows past 32) are whole 8- or 16-byte pieces
+// of memory, and 32 rows span 32 bits.
+bool rows_aligned(const Buf& b, int D) {
+  const int64_t elt = b.dt == TENSION_E4M3 ? 1 : b.dt == TENSION_F32 ? 4 : 2;
+  const int64_t to = b.dt == TENSION_E4M3 && D <= 32 ? 8 : 16;
+  return (uintptr_t)b.p % to == 0 && b.s0 * elt % to == 0 && b.s1 * elt % to == 0 && b.s2 * elt % to == 0 &&
+         b.s2 >= 0 && b.s2 < (1 << 24);
+}
+
+}  // namespace
+
+bool launch_paged_decode_rows(const PagedDecodeParams& p, hipStream_t st) {
+  if (p.D % 8 || !rows_aligned(p.c.k, p.D) || !rows_aligned(p.c.v, p.D)) return false;
+  if (p.c.ke2 < 0 || p.c.ke2 >= (1 << 24) || p.c.ve2 < 0 || p.c.ve2 >= (1 << 24)) return false;
+  constexpr int eight = 1024;
+  const int waves = (int64_t)p.N * p.Hk * p.splits < eight ? 8 : 4;
+  if (p.c.k.dt == TENSION_F32 && p.c.v.dt == TENSION_BF16) return launch_paged_rows_mixed(p, waves, st);
+  if (p.c.k.dt != p.c.v.dt) return false;
+  switch (p.c.k.dt) {
+    case TENSION_BF16: return launch_paged_rows_bf16(p, waves, st);
+    case TENSION_F16: return launch_paged_rows_f16(p, waves, st);
+    case TENSION_F32: return launch_paged_rows_f32(p, waves, st);
+    default: return launch_paged_rows_e4m3(p, waves, st);
+  }
+}
+
+}  // namespace tension
