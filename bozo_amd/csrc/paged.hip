@@ -123,8 +123,8 @@ __global__ void __launch_bounds__(kThreads) paged_rows_any(PagedRowsParams p) {
 
 struct VecGeometry {
   FastDiv heads, tiles, page;
-  int ntile, lg_tile;  // tiles of 2^lg_tile tokens of one sequence
-  int units;           // N * ntile * Hk * 2^lg_tile rows
+  int ntile;  // groups of R tokens of a sequence
+  int units;  // N * ntile * Hk: R tokens of one head
 };
 
 template <int CTRL>
@@ -150,133 +150,180 @@ __device__ __forceinline__ unsigned group_umax(unsigned x) {
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
-// Eight dense values as they are loaded, and as floats.
-template <bool F32>
+// The eight values of a lane, two groups of four: side by side, or, for
+// float32 dense rows, half a row apart, so that a wave's 16-byte accesses of
+// them cover whole lines.
+struct Quads {
+  int a, b;
+};
+template <bool F32, int LPR>
+__device__ __forceinline__ Quads lane_quads(int lane) {
+  return F32 ? Quads{4 * lane, 4 * LPR + 4 * lane} : Quads{8 * lane, 8 * lane + 4};
+}
+
+template <typename V>
+__device__ __forceinline__ void floats_as(u32x4 w, float* x) {
+  const V h = __builtin_bit_cast(V, w);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = (float)h[i];
+}
+template <typename V, typename T>
+__device__ __forceinline__ u32x4 rounded_as(const float* x) {
+  V h;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) h[i] = (T)x[i];
+  return __builtin_bit_cast(u32x4, h);
+}
+
+// Eight values of a row of float32 (WIDE) or 16-bit type, as they are loaded.
+template <bool WIDE>
 struct Eight {
-  u32x4 a[F32 ? 2 : 1];
-  __device__ __forceinline__ void load(const Buf& b, int64_t off) {
-    const u32x4* s = (const u32x4*)((const char*)b.p + off * (F32 ? 4 : 2));
-    a[0] = s[0];
-    if constexpr (F32) a[1] = s[1];
+  u32x4 a[WIDE ? 2 : 1];
+  __device__ __forceinline__ void load(const Buf& b, int64_t off, Quads q) {
+    if constexpr (WIDE) {
+      a[0] = *(const u32x4*)((const float*)b.p + off + q.a);
+      a[1] = *(const u32x4*)((const float*)b.p + off + q.b);
+    } else if (q.b == q.a + 4) {
+      a[0] = *(const u32x4*)((const f16*)b.p + off + q.a);
+    } else {
+      const u32x2 x = *(const u32x2*)((const f16*)b.p + off + q.a), y = *(const u32x2*)((const f16*)b.p + off + q.b);
+      a[0] = u32x4{x[0], x[1], y[0], y[1]};
+    }
   }
-  __device__ __forceinline__ void store(const Buf& b, int64_t off) const {
-    u32x4* s = (u32x4*)((char*)const_cast<void*>(b.p) + off * (F32 ? 4 : 2));
-    s[0] = a[0];
-    if constexpr (F32) s[1] = a[1];
+  __device__ __forceinline__ void store(const Buf& b, int64_t off, Quads q) const {
+    void* p = const_cast<void*>(b.p);
+    if constexpr (WIDE) {
+      *(u32x4*)((float*)p + off + q.a) = a[0];
+      *(u32x4*)((float*)p + off + q.b) = a[1];
+    } else if (q.b == q.a + 4) {
+      *(u32x4*)((f16*)p + off + q.a) = a[0];
+    } else {
+      *(u32x2*)((f16*)p + off + q.a) = u32x2{a[0][0], a[0][1]};
+      *(u32x2*)((f16*)p + off + q.b) = u32x2{a[0][2], a[0][3]};
+    }
   }
   __device__ __forceinline__ void floats(bool half, float* x) const {
-    if constexpr (F32) {
+    if constexpr (WIDE) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const unsigned w = a[i / 4][i % 4];  // a copy: bit_cast of a vector's element takes element 0
         x[i] = __builtin_bit_cast(float, w);
       }
     } else if (half) {
-      const f16x8 h = __builtin_bit_cast(f16x8, a[0]);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = (float)h[i];
+      floats_as<f16x8>(a[0], x);
     } else {
-      const bf16x8 h = __builtin_bit_cast(bf16x8, a[0]);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = (float)h[i];
+      floats_as<bf16x8>(a[0], x);
     }
   }
   __device__ __forceinline__ void set(bool half, const float* x) {
-    if constexpr (F32) {
+    if constexpr (WIDE) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) a[i / 4][i % 4] = __builtin_bit_cast(unsigned, x[i]);
     } else if (half) {
-      f16x8 h;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) h[i] = (f16)x[i];
-      a[0] = __builtin_bit_cast(u32x4, h);
+      a[0] = rounded_as<f16x8, f16>(x);
     } else {
-      bf16x8 h;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) h[i] = (bf16)x[i];
-      a[0] = __builtin_bit_cast(u32x4, h);
+      a[0] = rounded_as<bf16x8, bf16>(x);
     }
   }
 };
 
-// LPR lanes to a row, eight values to a lane, R rows to a thread (their loads
-// ahead of the first use).  A workgroup's consecutive rows are tokens of one
-// head: their places in a page lie together, and in the dense tensor each is a
-// piece of D values of its token.
+// The places of R consecutive tokens of one head.
+template <int R>
+struct Places {
+  int n, h, t, id[R], row[R];
+  bool in[R], live[R];  // the call's tokens; those with a place
+};
+
+// One side (K or V) of R rows: eight values to a lane, all loads ahead of the
+// first use.
 template <bool APPEND, int LPR, int R, bool F32>
-__device__ __forceinline__ void vec_rows(const PagedRowsParams& p, const VecGeometry& g, bool isv) {
-  constexpr int kRows = kThreads / LPR;
-  const Buf& pg = isv ? p.c.v : p.c.k;
-  const Buf& de = isv ? p.vd : p.kd;
-  uint8_t* ex = const_cast<uint8_t*>(isv ? p.c.ve : p.c.ke);
-  const int64_t e0 = isv ? p.c.ve0 : p.c.ke0, e1 = isv ? p.c.ve1 : p.c.ke1, e2 = isv ? p.c.ve2 : p.c.ke2;
-  const int ch = threadIdx.x % LPR * 8;
-  int64_t doff[R], poff[R], eoff[R];
-  bool live[R], in[R];
+struct Side {
   Eight<F32> x[R];
+  u32x2 c[R];
+  uint8_t b[R];
+
+  static __device__ __forceinline__ int64_t page_off(const Buf& pg, const Places<R>& w, int r) {
+    return w.id[r] * pg.s0 + w.h * pg.s1 + w.row[r] * pg.s2;
+  }
+
+  __device__ __forceinline__ void load(const Buf& de, const Buf& pg, const uint8_t* ex, int64_t e0, int64_t e1, int64_t e2,
+                                       const Places<R>& w, int lane) {
+    const Quads q = lane_quads<F32, LPR>(lane);
+    if constexpr (APPEND) {
+      const int64_t off = w.n * de.s0 + w.t * de.s1 + w.h * de.s2;
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int u = (blockIdx.x * R + r) * kRows + threadIdx.x / LPR;
-    const int y = u >> g.lg_tile, z = fdiv(y, g.heads), h = y - z * p.Hk;
-    const int n = fdiv(z, g.tiles), t = ((z - n * g.ntile) << g.lg_tile) + (u & ((1 << g.lg_tile) - 1));
-    in[r] = u < g.units && t < p.T;
-    doff[r] = n * de.s0 + t * de.s1 + h * de.s2 + ch;
-    live[r] = false;
-    int pos = 0;
-    if (in[r] && token_pos(p, n, t, &pos)) {
-      const int slot = fdiv(pos, g.page), row = pos - slot * p.c.S;
-      if (APPEND) x[r].load(de, doff[r]);
-      if (slot < p.c.table_len) {
-        const int id = p.c.table[(int64_t)n * p.c.table_stride + slot];
-        live[r] = id >= 0 && id < p.c.P;
-        poff[r] = id * pg.s0 + h * pg.s1 + row * pg.s2 + ch;
-        eoff[r] = id * e0 + h * e1 + row * e2;
+      for (int r = 0; r < R; ++r)
+        if (w.live[r]) x[r].load(de, off + r * de.s1, q);
+      return;
+    }
+    if (pg.dt == TENSION_E4M3) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const uint8_t* s = (const uint8_t*)pg.p + (w.live[r] ? page_off(pg, w, r) : 0);
+        if constexpr (F32)
+          c[r] = u32x2{w.live[r] ? *(const unsigned*)(s + q.a) : 0, w.live[r] ? *(const unsigned*)(s + q.b) : 0};
+        else
+          c[r] = w.live[r] ? *(const u32x2*)(s + q.a) : u32x2{0, 0};
+        b[r] = w.live[r] ? ex[w.id[r] * e0 + w.h * e1 + w.row[r] * e2] : 127;
+      }
+    } else if (pg.dt == de.dt) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float zero[8] = {};
+        x[r].set(false, zero);
+        if (w.live[r]) x[r].load(pg, page_off(pg, w, r), q);
       }
     }
   }
-  const bool half = de.dt == TENSION_F16, quantised = pg.dt == TENSION_E4M3;
-  if constexpr (APPEND) {
+
+  __device__ __forceinline__ void store(const Buf& de, const Buf& pg, uint8_t* ex, int64_t e0, int64_t e1, int64_t e2,
+                                        const Places<R>& w, int lane) {
+    const Quads q = lane_quads<F32, LPR>(lane);
+    const bool half = de.dt == TENSION_F16;
+    if constexpr (APPEND) {
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      if (!live[r]) continue;  // a row's lanes agree
-      if (!quantised) {
+      for (int r = 0; r < R; ++r) {
+        if (!w.live[r]) continue;  // a row's lanes agree
+        const int64_t off = page_off(pg, w, r);
         if (pg.dt == de.dt) {
-          x[r].store(pg, poff[r]);
-        } else {  // float32 tokens, 16-bit pages
-          float f[8];
-          x[r].floats(half, f);
+          x[r].store(pg, off, q);
+          continue;
+        }
+        float f[8];
+        x[r].floats(half, f);
+        if (pg.dt != TENSION_E4M3) {  // float32 tokens, 16-bit pages
           Eight<false> y;
           y.set(pg.dt == TENSION_F16, f);
-          y.store(pg, poff[r]);
+          y.store(pg, off, q);
+          continue;
         }
-        continue;
-      }
-      float f[8];
-      x[r].floats(half, f);
-      unsigned top = 0;
+        unsigned top = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const unsigned b = finite_bits(f[i]);
-        top = b > top ? b : top;
-      }
-      const int b = exp_byte(group_umax<LPR>(top));
-      const float inv = pow2_of_byte(254 - b);
+        for (int i = 0; i < 8; ++i) {
+          const unsigned m = finite_bits(f[i]);
+          top = m > top ? m : top;
+        }
+        const int e = exp_byte(group_umax<LPR>(top));
+        const float inv = pow2_of_byte(254 - e);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = to_code_range(f[i], inv);
-      *(u32x2*)((uint8_t*)pg.p + poff[r]) = u32x2{pack4(f[0], f[1], f[2], f[3]), pack4(f[4], f[5], f[6], f[7])};
-      if (ch == 0) ex[eoff[r]] = (uint8_t)b;
+        for (int i = 0; i < 8; ++i) f[i] = to_code_range(f[i], inv);
+        const u32x2 codes = {pack4(f[0], f[1], f[2], f[3]), pack4(f[4], f[5], f[6], f[7])};
+        uint8_t* to = (uint8_t*)pg.p + off;
+        if constexpr (F32) {
+          *(unsigned*)(to + q.a) = codes[0];
+          *(unsigned*)(to + q.b) = codes[1];
+        } else {
+          *(u32x2*)(to + q.a) = codes;
+        }
+        if (lane == 0) ex[w.id[r] * e0 + w.h * e1 + w.row[r] * e2] = (uint8_t)e;
+      }
+      return;
     }
-  } else {
-    if (quantised) {
-      u32x2 c[R];
-      uint8_t b[R];
+    const int64_t off = w.n * de.s0 + w.t * de.s1 + w.h * de.s2;
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        c[r] = live[r] ? *(const u32x2*)((const uint8_t*)pg.p + poff[r]) : u32x2{0, 0};
-        b[r] = live[r] ? ex[eoff[r]] : 127;
-      }
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
+    for (int r = 0; r < R; ++r) {
+      if (!w.in[r]) continue;
+      if (pg.dt == TENSION_E4M3) {
         float f[8];
         const float s = pow2_of_byte(b[r]);
 #pragma unroll
@@ -287,41 +334,64 @@ __device__ __forceinline__ void vec_rows(const PagedRowsParams& p, const VecGeom
           f[4 * i + 3] = __builtin_amdgcn_cvt_f32_fp8((int)c[r][i], 3) * s;
         }
         x[r].set(half, f);
-        if (in[r]) x[r].store(de, doff[r]);
-      }
-      return;
-    }
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      if (!in[r]) continue;
-      float f[8] = {};
-      if (!live[r]) {
-        x[r].set(half, f);
-      } else if (pg.dt == de.dt) {
-        x[r].load(pg, poff[r]);
-      } else if (pg.dt == TENSION_F32) {
-        Eight<true> y;
-        y.load(pg, poff[r]);
-        y.floats(false, f);
-        x[r].set(half, f);
-      } else {
-        Eight<false> y;
-        y.load(pg, poff[r]);
-        y.floats(pg.dt == TENSION_F16, f);
+      } else if (pg.dt != de.dt) {
+        float f[8] = {};
+        if (w.live[r]) {
+          const int64_t from = page_off(pg, w, r);
+          if (pg.dt == TENSION_F32) {
+            Eight<true> y;
+            y.load(pg, from, q);
+            y.floats(false, f);
+          } else {
+            Eight<false> y;
+            y.load(pg, from, q);
+            y.floats(pg.dt == TENSION_F16, f);
+          }
+        }
         x[r].set(half, f);
       }
-      x[r].store(de, doff[r]);
+      x[r].store(de, off + r * de.s1, q);
     }
   }
-}
+};
 
-template <bool APPEND, int LPR, int R>
+// LPR lanes to a row, R tokens of one head to a thread, K and V both.
+// Consecutive units are heads of one token, so a wave's rows lie together in
+// the dense tensors, and a thread's tokens lie together in a page.
+template <bool APPEND, int LPR, int R, bool KF32, bool VF32>
 __global__ void __launch_bounds__(kThreads) paged_rows_vec(PagedRowsParams p, VecGeometry g) {
-  const bool isv = blockIdx.y != 0;
-  if ((isv ? p.vd.dt : p.kd.dt) == TENSION_F32)
-    vec_rows<APPEND, LPR, R, true>(p, g, isv);
-  else
-    vec_rows<APPEND, LPR, R, false>(p, g, isv);
+  const int lane = threadIdx.x % LPR;
+  const int u = blockIdx.x * (kThreads / LPR) + threadIdx.x / LPR;
+  if (u >= g.units) return;
+  Places<R> w;
+  const int y = fdiv(u, g.heads);
+  w.h = u - y * p.Hk;
+  w.n = fdiv(y, g.tiles);
+  w.t = (y - w.n * g.ntile) * R;
+  const int64_t first = (int64_t)p.start[w.n] + w.t;
+  const int count = p.counts ? p.counts[w.n] : p.T;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int64_t pos = first + r;
+    w.in[r] = w.t + r < p.T;
+    w.live[r] = false;
+    w.id[r] = w.row[r] = 0;
+    if (w.in[r] && w.t + r < count && pos >= 0 && pos <= 0x7fffffff) {
+      const int slot = fdiv((int)pos, g.page);
+      if (slot < p.c.table_len) {
+        w.id[r] = p.c.table[(int64_t)w.n * p.c.table_stride + slot];
+        w.row[r] = (int)pos - slot * p.c.S;
+        w.live[r] = w.id[r] >= 0 && w.id[r] < p.c.P;
+      }
+    }
+  }
+  Side<APPEND, LPR, R, KF32> k;
+  Side<APPEND, LPR, R, VF32> v;
+  uint8_t *ke = const_cast<uint8_t*>(p.c.ke), *ve = const_cast<uint8_t*>(p.c.ve);
+  k.load(p.kd, p.c.k, ke, p.c.ke0, p.c.ke1, p.c.ke2, w, lane);
+  v.load(p.vd, p.c.v, ve, p.c.ve0, p.c.ve1, p.c.ve2, w, lane);
+  k.store(p.kd, p.c.k, ke, p.c.ke0, p.c.ke1, p.c.ke2, w, lane);
+  v.store(p.vd, p.c.v, ve, p.c.ve0, p.c.ve1, p.c.ve2, w, lane);
 }
 
 // Pieces of 8 values of a row are whole 16-byte (8-byte: e4m3) pieces of memory.
@@ -330,12 +400,20 @@ bool vec_aligned(const Buf& b) {
   return (uintptr_t)b.p % to == 0 && b.s0 * bytes % to == 0 && b.s1 * bytes % to == 0 && b.s2 * bytes % to == 0;
 }
 
-template <bool APPEND, int R>
-bool launch_vec(const PagedRowsParams& p, const VecGeometry& g, hipStream_t st) {
+template <bool APPEND, int R, bool KF32, bool VF32>
+bool launch_vec(const PagedRowsParams& p, hipStream_t st) {
+  VecGeometry g;
+  g.ntile = (p.T + R - 1) / R;
+  const int64_t units = mul_cap((int64_t)p.N * g.ntile, p.Hk, 1 << 30);
+  if (units < 0) return false;
+  g.units = (int)units;
+  g.heads = fast_div(p.Hk);
+  g.tiles = fast_div(g.ntile);
+  g.page = fast_div(p.c.S);
   auto go = [&](auto lanes) {
     constexpr int LPR = decltype(lanes)::value;
-    const int per = kThreads / LPR * R;
-    paged_rows_vec<APPEND, LPR, R><<<dim3((unsigned)((g.units + per - 1) / per), 2), kThreads, 0, st>>>(p, g);
+    const int per = kThreads / LPR;
+    paged_rows_vec<APPEND, LPR, R, KF32, VF32><<<(unsigned)((g.units + per - 1) / per), kThreads, 0, st>>>(p, g);
     return true;
   };
   switch (p.D) {
@@ -347,23 +425,22 @@ bool launch_vec(const PagedRowsParams& p, const VecGeometry& g, hipStream_t st) 
   }
 }
 
+template <bool APPEND, int R>
+bool launch_types(const PagedRowsParams& p, hipStream_t st) {
+  const bool k = p.kd.dt == TENSION_F32, v = p.vd.dt == TENSION_F32;
+  if (k) return v ? launch_vec<APPEND, R, true, true>(p, st) : launch_vec<APPEND, R, true, false>(p, st);
+  return v ? launch_vec<APPEND, R, false, true>(p, st) : launch_vec<APPEND, R, false, false>(p, st);
+}
+
 // Head dims 32 to 256 (powers of two) with aligned rows.
 bool try_vec(bool append, const PagedRowsParams& p, hipStream_t st) {
   if (!vec_aligned(p.kd) || !vec_aligned(p.vd) || !vec_aligned(p.c.k) || !vec_aligned(p.c.v)) return false;
-  VecGeometry g;
-  g.lg_tile = 0;
-  while (g.lg_tile < 5 && (1 << g.lg_tile) < p.T) ++g.lg_tile;
-  g.ntile = (int)(((int64_t)p.T + (1 << g.lg_tile) - 1) >> g.lg_tile);
-  const int64_t units = mul_cap(mul_cap((int64_t)p.N * g.ntile, p.Hk, 1 << 30), (int64_t)1 << g.lg_tile, 1 << 30);
-  if (units < 0) return false;
-  g.units = (int)units;
-  g.heads = fast_div(p.Hk);
-  g.tiles = fast_div(g.ntile);
-  g.page = fast_div(p.c.S);
-  // several rows to a thread once the grid fills the card many times over
-  const bool many = units * (p.D / 8) >= (int64_t)kThreads * device_cus() * 32;
-  if (append) return many ? launch_vec<true, 4>(p, g, st) : launch_vec<true, 1>(p, g, st);
-  return many ? launch_vec<false, 4>(p, g, st) : launch_vec<false, 1>(p, g, st);
+  const int64_t threads = mul_cap((int64_t)p.N * p.T, (int64_t)p.Hk * p.D / 8, (int64_t)1 << 40);
+  // Two tokens to a thread for reads that fill the card more than once (E4M3 to bf16, N8 Hk16 D64: T1024 12.6 -> 10.4
+  // us, T4096 52.6 -> 40.4; T256 5.9 either way); four were no faster (41.8), and appending was fastest with one.
+  const bool two = threads < 0 || threads >= (int64_t)kThreads * device_cus() * 8;
+  if (append) return launch_types<true, 1>(p, st);
+  return two ? launch_types<false, 2>(p, st) : launch_types<false, 1>(p, st);
 }
 
 }  // namespace
