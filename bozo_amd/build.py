@@ -27,7 +27,7 @@ HOSTNAME = "_host.so"
 ARCH = os.environ.get("TENSION_OFFLOAD_ARCH", "gfx950")
 
 SOURCES = [
-    "capi.hip", "exact.hip", "decode.hip", "paged.hip", "paged_decode.hip", "paged_decode_rows.hip",
+    "capi.hip", "exact.hip", "decode.hip", "paged.hip", "paged_decode.hip", "paged_decode_rows.hip", "paged_decode_mfma.hip",
     "paged_rows_bf16.hip", "paged_rows_f16.hip", "paged_rows_f32.hip", "paged_rows_mixed.hip", "paged_rows_e4m3.hip",
     "mfma.hip", "mfma_fwd.hip", "mfma_dq.hip", "mfma_dkv.hip", "mfma_bwd_fused.hip", "mfma_global.hip",
     "mfma_wide.hip",

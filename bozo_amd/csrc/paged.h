@@ -67,5 +67,6 @@ __device__ __forceinline__ float pow2_of_byte(int b) { return __builtin_bit_cast
 // Kernels for whole 16-byte pieces of a row.  False when the call has no such
 // form; the caller then runs the kernel for any.
 bool launch_paged_decode_rows(const PagedDecodeParams& p, hipStream_t st);
+bool launch_paged_decode_mfma(const PagedDecodeParams& p, hipStream_t st);
 
 }  // namespace tension

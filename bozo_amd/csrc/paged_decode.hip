@@ -120,10 +120,13 @@ void launch_join(const PagedDecodeParams& p, hipStream_t st) {
 
 }  // namespace
 
-// About four workgroups per CU (all of them resident), splits of 128 keys at
-// least.
+// About as many workgroups as are resident together, so that one round takes
+// them all: four per CU, two where the matrix kernel holds head dim 128 (e4m3,
+// 8 rows of 65500 keys: 512 workgroups 30 us, 768 31, 1024 33).  Splits of 128
+// keys at least.
 void paged_decode_split(int64_t N, int64_t H, int64_t Hk, int64_t D, int64_t W, int64_t max_len, int* splits, int* chunk) {
-  constexpr int target = 1024, least = 128;
+  constexpr int least = 128;
+  const int target = H > Hk && D > 64 ? 512 : 1024;
   const int64_t keys = W > 0 && W + 1 < max_len ? W + 1 : max_len;
   const int64_t rows = N * Hk;
   int64_t ns = (target + rows / 2) / (rows > 0 ? rows : 1);
