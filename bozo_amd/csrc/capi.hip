@@ -846,9 +846,9 @@ int paged_rows(bool append, const tension_paged* cache, const tension_buf* k, co
   return launched(e, what);
 }
 
-// Sizes of a decode call; the bound of the lengths that shapes the launch.
+// Sizes of a decode call; the keys of a sequence that shape the launch.
 int paged_decode_sizes(int64_t N, int64_t H, int64_t Hk, int64_t D, int64_t W, int64_t max_len, int64_t table_len,
-                       int64_t page_size, int64_t* bound) {
+                       int64_t page_size, int64_t* keys) {
   if (N < 0 || H < 0 || Hk < 0 || D < 1 || D > 256 || W < 0 || W > 0x3fffffff || max_len < 0 || table_len < 0 ||
       table_len > 0x7fffffff || page_size < 1 || page_size > 0x3fffffff || mul_cap(N, H, 0x7fffff) < 0 ||
       (H > 0 && (Hk < 1 || H % Hk)))
@@ -858,7 +858,8 @@ int paged_decode_sizes(int64_t N, int64_t H, int64_t Hk, int64_t D, int64_t W, i
                 (long long)table_len, (long long)page_size);
   int64_t cap = mul_cap(table_len, page_size, 0x7fffffff);
   if (cap < 0) cap = 0x7fffffff;
-  *bound = max_len > 0 && max_len < cap ? max_len : cap;
+  *keys = max_len > 0 && max_len < cap ? max_len : cap;
+  if (W > 0 && W + 1 < *keys) *keys = W + 1;
   return 0;
 }
 
@@ -878,18 +879,18 @@ int tension_paged_read(const tension_paged* cache, const tension_buf* k_out, con
 
 int64_t tension_paged_decode_workspace(int64_t N, int64_t H, int64_t Hk, int64_t D, int64_t W, int64_t max_len,
                                        int64_t table_len, int64_t page_size) {
-  int64_t bound = 0;
-  if (paged_decode_sizes(N, H, Hk, D, W, max_len, table_len, page_size, &bound)) return -1;
+  int64_t keys = 0;
+  if (paged_decode_sizes(N, H, Hk, D, W, max_len, table_len, page_size, &keys)) return -1;
   int splits = 1, chunk = 0;
-  if (N * H > 0) paged_decode_split(N, H, Hk, D, W, bound, &splits, &chunk);
+  if (N * H > 0) paged_decode_split(N, H, Hk, D, keys, &splits, &chunk);
   return splits > 1 ? N * H * splits * (D + 1) * (int64_t)sizeof(float) : 0;
 }
 
 int tension_paged_decode(const tension_paged* cache, const tension_buf* q, const tension_buf* out,
                          const int32_t* lengths, void* workspace, int64_t N, int64_t H, int64_t Hk, int64_t D,
                          int64_t W, int64_t max_len, double scale, int32_t flags, tension_stream_t stream) {
-  int64_t bound = 0;
-  TRY(paged_decode_sizes(N, H, Hk, D, W, max_len, cache ? cache->table_len : 0, cache ? cache->page_size : 1, &bound));
+  int64_t keys = 0;
+  TRY(paged_decode_sizes(N, H, Hk, D, W, max_len, cache ? cache->table_len : 0, cache ? cache->page_size : 1, &keys));
   if (!(std::isfinite(scale) && scale != 0.0)) return fail(TENSION_ERR_ARG, "scale must be finite and non-zero");
   if (N * H == 0) return ok();
   PagedDecodeParams p;
@@ -904,7 +905,8 @@ int tension_paged_decode(const tension_paged* cache, const tension_buf* q, const
   p.q = make_buf(q); p.out = make_buf(out); p.lengths = lengths; p.ws = (float*)workspace;
   p.N = (int)N; p.H = (int)H; p.Hk = (int)Hk; p.D = (int)D; p.W = (int)W;
   p.scale = (float)scale; p.inv_scale = (float)(1.0 / scale); p.flags = flags;
-  paged_decode_split(N, H, Hk, D, W, bound, &p.splits, &p.chunk);
+  p.most = keys;
+  paged_decode_split(N, H, Hk, D, keys, &p.splits, &p.chunk);
   if (p.splits > 1 && !workspace) return fail(TENSION_ERR_ARG, "paged decode: workspace is required");
   hipError_t e = hipSuccess;
   launch_paged_decode(p, hs(stream), &e);

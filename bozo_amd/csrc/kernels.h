@@ -99,13 +99,14 @@ struct PagedDecodeParams {
   float* ws;   // [N * H, splits, D + 1] partial sums and masses, null when splits == 1
   int N, H, Hk, D, W;
   int splits, chunk;  // split i: keys from lo + i * chunk, the last one to the end
+  int64_t most;       // keys of a sequence, as the launch is shaped
   float scale, inv_scale;
   int flags;
 };
 
-// Keys per split and splits of a decode call (one rule for the workspace
-// query and the launch).
-void paged_decode_split(int64_t N, int64_t H, int64_t Hk, int64_t D, int64_t W, int64_t max_len, int* splits, int* chunk);
+// Splits of a decode call over at most `keys` keys a sequence, and keys per
+// split (one rule for the workspace query and the launch).
+void paged_decode_split(int64_t N, int64_t H, int64_t Hk, int64_t D, int64_t keys, int* splits, int* chunk);
 int launch_paged_rows(bool append, const PagedRowsParams& p, hipStream_t st, hipError_t* err);
 int launch_paged_decode(const PagedDecodeParams& p, hipStream_t st, hipError_t* err);
 

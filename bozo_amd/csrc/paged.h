@@ -64,6 +64,31 @@ __device__ __forceinline__ float* split_mass(const PagedDecodeParams& p, int nh,
 // Scale of an exponent byte.
 __device__ __forceinline__ float pow2_of_byte(int b) { return __builtin_bit_cast(float, (unsigned)b << 23); }
 
+// Workgroups of a decode call: (sequence, key head, group of query heads, split).
+struct DecodeGrid {
+  FastDiv page, dim, splits, heads, group_div;
+  int share, groups;  // query heads of a key head, and their groups
+
+  DecodeGrid(const PagedDecodeParams& p, int per_group) {
+    share = p.H / p.Hk;
+    groups = (share + per_group - 1) / per_group;
+    page = fast_div(p.c.S);
+    dim = fast_div(p.D);
+    splits = fast_div(p.splits);
+    heads = fast_div(p.Hk);
+    group_div = fast_div(groups);
+  }
+  unsigned size(const PagedDecodeParams& p) const { return (unsigned)((int64_t)p.N * p.Hk * groups * p.splits); }
+  __device__ __forceinline__ void place(int b, const PagedDecodeParams& p, int* n, int* hk, int* grp, int* split) const {
+    int x = fdiv(b, splits);
+    *split = b - x * p.splits;
+    int y = fdiv(x, group_div);
+    *grp = x - y * groups;
+    *n = fdiv(y, heads);
+    *hk = y - *n * p.Hk;
+  }
+};
+
 // Kernels for whole 16-byte pieces of a row.  False when the call has no such
 // form; the caller then runs the kernel for any.
 bool launch_paged_decode_rows(const PagedDecodeParams& p, hipStream_t st);

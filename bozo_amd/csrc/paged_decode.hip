@@ -120,18 +120,29 @@ void launch_join(const PagedDecodeParams& p, hipStream_t st) {
 
 }  // namespace
 
-// About as many workgroups as are resident together, so that one round takes
-// them all: four per CU, two where the matrix kernel holds head dim 128 (e4m3,
-// 8 rows of 65500 keys: 512 workgroups 30 us, 768 31, 1024 33).  Splits of 128
-// keys at least.
-void paged_decode_split(int64_t N, int64_t H, int64_t Hk, int64_t D, int64_t W, int64_t max_len, int* splits, int* chunk) {
-  constexpr int least = 128;
-  const int target = H > Hk && D > 64 ? 512 : 1024;
-  const int64_t keys = W > 0 && W + 1 < max_len ? W + 1 : max_len;
-  const int64_t rows = N * Hk;
-  int64_t ns = (target + rows / 2) / (rows > 0 ? rows : 1);
-  const int64_t most = keys / least;
-  ns = ns > most ? most : ns;
+// Splits of a sequence's keys.  A CU streams about 25 KB/us of cache whether
+// one workgroup or four run on it, so a call takes as long as its fullest CU;
+// the partial sums and the second kernel cost about 3 us more.  Tried: one
+// split, and what fills the CUs one to four times (two where the matrix kernel
+// holds head dim 128), with 128 keys to a split at least.
+void paged_decode_split(int64_t N, int64_t H, int64_t Hk, int64_t D, int64_t keys, int* splits, int* chunk) {
+  constexpr float kBytesPerUs = 25e3f, kJoinUs = 3.f;
+  constexpr int64_t kLeast = 128;
+  const int64_t rows = N * Hk, cus = device_cus();
+  const float row_us = (float)keys * (float)(4 * D) / kBytesPerUs;
+  const int fills = H > Hk && D > 64 ? 2 : 4;
+  float best = (float)((rows + cus - 1) / cus) * row_us;
+  int64_t ns = 1;
+  for (int f = 1; f <= fills; ++f) {
+    int64_t s = rows > 0 ? f * cus / rows : 1;
+    s = s < keys / kLeast ? s : keys / kLeast;
+    if (s <= ns) continue;
+    const float t = (float)((rows * s + cus - 1) / cus) / (float)s * row_us + kJoinUs;
+    if (t < best) {
+      best = t;
+      ns = s;
+    }
+  }
   if (ns <= 1) {
     *splits = 1;
     *chunk = 0x40000000;

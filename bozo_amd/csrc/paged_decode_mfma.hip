@@ -61,10 +61,9 @@ __device__ __forceinline__ unsigned halves(unsigned a, unsigned b) {
 }
 
 // F8: e4m3 pages, else bf16.  QF16: queries are f16 (F8 only).
-template <bool F8, bool QF16, int D>
-__global__ void __launch_bounds__(256, F8 || D == 64 ? 3 : 2) paged_decode_mfma(PagedDecodeParams p, FastDiv page_div) {
+template <bool F8, bool QF16, int D, int kWaves>
+__global__ void __launch_bounds__(64 * kWaves, F8 || D == 64 ? 3 : 2) paged_decode_mfma(PagedDecodeParams p, DecodeGrid grid) {
   constexpr int kElt = F8 ? 1 : 2;
-  constexpr int kWaves = 4;
   constexpr int KP = D * kElt / 64;      // 16-byte pieces a lane loads of a tile's K: 64 bytes of a row each
   constexpr int KS = D / 32;             // products of a tile's scores
   constexpr int VN = D / 16;             // values of a lane's piece of a V row
@@ -72,14 +71,9 @@ __global__ void __launch_bounds__(256, F8 || D == 64 ? 3 : 2) paged_decode_mfma(
   __shared__ float red[kWaves][16][D + 1];
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int share = p.H / p.Hk, groups = (share + 15) / 16;
-  int b = (int)blockIdx.x;
-  const int split = b % p.splits;
-  b /= p.splits;
-  const int grp = b % groups;
-  b /= groups;
-  const int hk = b % p.Hk, n = b / p.Hk;
-  const int h0 = hk * share + grp * 16, nh = share - grp * 16 < 16 ? share - grp * 16 : 16;
+  int n, hk, grp, split;
+  grid.place((int)blockIdx.x, p, &n, &hk, &grp, &split);
+  const int h0 = hk * grid.share + grp * 16, nh = grid.share - grp * 16 < 16 ? grid.share - grp * 16 : 16;
   const KeyRange all = key_range(p, n), r = split_range(p, all, split);
   if (p.splits > 1 && split >= used_splits(p, all)) return;
 
@@ -100,7 +94,7 @@ __global__ void __launch_bounds__(256, F8 || D == 64 ? 3 : 2) paged_decode_mfma(
   auto where = [&](int64_t base, int t, int* id, int* row) {
     const unsigned pos = (unsigned)base + t * kTileKeys, hi = (unsigned)r.hi;
     const int at = pos < hi ? (int)pos : r.hi - 1;
-    const int slot = fdiv(at, page_div);
+    const int slot = fdiv(at, grid.page);
     const int x = table[slot];
     *row = pos < hi ? at - slot * p.c.S : 0;  // a tile past the end reads its page's first
     page_ok[t] = x >= 0 && x < p.c.P;
@@ -263,7 +257,7 @@ __global__ void __launch_bounds__(256, F8 || D == 64 ? 3 : 2) paged_decode_mfma(
     for (int i = 0; i < 4; ++i) red[wave][4 * g + i][c * VN + j] = acc[j][i];
   if (g == 0) red[wave][c][D] = mass;
   __syncthreads();
-  for (int i = tid; i < nh * D; i += 256) {
+  for (int i = tid; i < nh * D; i += 64 * kWaves) {
     const int h = i / D, d = i % D;
     float o = 0.f, m = 0.f;
 #pragma unroll
@@ -283,11 +277,16 @@ __global__ void __launch_bounds__(256, F8 || D == 64 ? 3 : 2) paged_decode_mfma(
 
 template <bool F8, bool QF16>
 void launch_as(const PagedDecodeParams& p, hipStream_t st) {
-  const unsigned grid = (unsigned)((int64_t)p.N * p.Hk * ((p.H / p.Hk + 15) / 16) * p.splits);
+  const DecodeGrid grid(p, 16);
+  const unsigned n = grid.size(p);
+  // eight waves where a CU has one workgroup
+  const bool eight = n <= (unsigned)device_cus();
   if (p.D == 64)
-    paged_decode_mfma<F8, QF16, 64><<<grid, 256, 0, st>>>(p, fast_div(p.c.S));
+    eight ? paged_decode_mfma<F8, QF16, 64, 8><<<n, 512, 0, st>>>(p, grid)
+          : paged_decode_mfma<F8, QF16, 64, 4><<<n, 256, 0, st>>>(p, grid);
   else
-    paged_decode_mfma<F8, QF16, 128><<<grid, 256, 0, st>>>(p, fast_div(p.c.S));
+    eight ? paged_decode_mfma<F8, QF16, 128, 8><<<n, 512, 0, st>>>(p, grid)
+          : paged_decode_mfma<F8, QF16, 128, 4><<<n, 256, 0, st>>>(p, grid);
 }
 
 }  // namespace

@@ -20,6 +20,19 @@ bool rows_aligned(const Buf& b, int D) {
          b.s2 >= 0 && b.s2 < (1 << 24);
 }
 
+// Waves of a workgroup.  Up to one workgroup per CU the call waits for memory
+// (N16 H12, 1000 bf16 keys: eight waves 10.2 us, four 12.3), and where each
+// takes long the last to end count (N128 H16, up to 4096 ragged: 212 against
+// 219).  Windows of two batches of a pair of waves leave the others nothing
+// (N128 H16 W64 e4m3: two waves 8.3 us, four 10.6).
+int waves_for(const PagedDecodeParams& p) {
+  const int64_t groups = (int64_t)p.N * p.Hk * p.splits, cus = device_cus();
+  const int64_t keys = p.splits > 1 ? p.chunk : p.most;
+  if (groups <= cus) return keys > 64 ? 8 : 4;
+  if (keys <= 128) return groups >= 3 * cus ? 2 : 4;
+  return keys >= 2048 ? 8 : 4;
+}
+
 }  // namespace
 
 bool launch_paged_decode_rows(const PagedDecodeParams& p, hipStream_t st) {
@@ -28,8 +41,7 @@ bool launch_paged_decode_rows(const PagedDecodeParams& p, hipStream_t st) {
   // A shared key head on the matrix units where its types allow: two query heads cost the same either way (bf16 D64,
   // 268 MB: 48 us), four 48.8 against 59.0 us, eight 50 against 102; e4m3 D128, 135 MB, four heads 30 against 50 us.
   if (p.H / p.Hk >= 2 && launch_paged_decode_mfma(p, st)) return true;
-  constexpr int eight = 1024;
-  const int waves = (int64_t)p.N * p.Hk * p.splits < eight ? 8 : 4;
+  const int waves = waves_for(p);
   if (p.c.k.dt == TENSION_F32 && p.c.v.dt == TENSION_BF16) return launch_paged_rows_mixed(p, waves, st);
   if (p.c.k.dt != p.c.v.dt) return false;
   switch (p.c.k.dt) {

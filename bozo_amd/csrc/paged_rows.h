@@ -92,13 +92,47 @@ __device__ __forceinline__ float row_sum(float x) {
   return x;
 }
 
-// Sum over the lanes with the same lane % LPR, on the first LPR lanes at least.
-template <int LPR>
-__device__ __forceinline__ float column_sum(float x) {
+// Sums over the lanes with the same lane % LPR of a lane's N values x: halves
+// of the wave trade one value of a pair for the other and add, then rows of 16
+// do, so that value kept(lane, j) ends up in x[j], j < N / kParts, of the lanes
+// that write().
+template <int LPR, int N>
+struct Fold {
+  static constexpr int kParts = LPR == 32 ? 2 : 4;
+  static __device__ __forceinline__ int kept(int lane, int j) {
+    return LPR == 32 ? 2 * j + lane / 32 : 4 * j + 2 * (lane / 16 % 2) + lane / 32;
+  }
+  static __device__ __forceinline__ bool write(int lane) { return LPR >= 16 || lane % 16 < LPR; }
+  static __device__ __forceinline__ float in_row(float x) {
+    if constexpr (LPR <= 8) x += dpp_move<0x128>(x);  // lane - 8 of its row
+    if constexpr (LPR <= 4) x += dpp_move<0x124>(x);  // lane - 4
+    return x;
+  }
+  static __device__ __forceinline__ float add_halves(float a, float b) {
+    const auto w = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b), false, false);
+    const unsigned lo = w[0], hi = w[1];
+    return __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
+  }
+  static __device__ __forceinline__ float add_rows(float a, float b) {
+    const auto w = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b), false, false);
+    const unsigned lo = w[0], hi = w[1];
+    return __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
+  }
+  static __device__ __forceinline__ void run(float* x) {
 #pragma unroll
-  for (int m = LPR; m < 64; m <<= 1) x += __shfl_xor(x, m);
-  return x;
-}
+    for (int i = 0; i < N / 2; ++i) x[i] = add_halves(x[2 * i], x[2 * i + 1]);
+    if constexpr (LPR < 32) {
+#pragma unroll
+      for (int i = 0; i < N / 4; ++i) x[i] = in_row(add_rows(x[2 * i], x[2 * i + 1]));
+    }
+  }
+  // Of one value, on every lane.
+  static __device__ __forceinline__ float sum(float x) {
+    x = add_halves(x, x);
+    if constexpr (LPR < 32) x = in_row(add_rows(x, x));
+    return x;
+  }
+};
 
 // The lane's values of G query rows, in the order of its K values.
 template <int KD, int VPL, int LPR, int G>
@@ -159,7 +193,7 @@ struct Query {
 };
 
 template <int KD, int VD, int VPL, int LPR, int G, int U, bool ALIGNED>
-__global__ void __launch_bounds__(512) paged_decode_rows(PagedDecodeParams p, FastDiv page_div) {
+__global__ void __launch_bounds__(G == 1 ? 1024 : 512) paged_decode_rows(PagedDecodeParams p, DecodeGrid grid) {
   constexpr int RPW = 64 / LPR;
   constexpr bool KE = KD == TENSION_E4M3, VE = VD == TENSION_E4M3;
   using PK = Piece<KD, VPL, LPR>;
@@ -167,14 +201,9 @@ __global__ void __launch_bounds__(512) paged_decode_rows(PagedDecodeParams p, Fa
   extern __shared__ float red[];  // [waves][G][D + 1]
   const int tid = threadIdx.x, lane = tid & 63, ch = lane % LPR, lr = lane / LPR;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = (int)blockDim.x >> 6;
-  const int share = p.H / p.Hk, groups = (share + G - 1) / G;
-  int b = (int)blockIdx.x;
-  const int split = b % p.splits;
-  b /= p.splits;
-  const int grp = b % groups;
-  b /= groups;
-  const int hk = b % p.Hk, n = b / p.Hk;
-  const int h0 = hk * share + grp * G, nh = share - grp * G < G ? share - grp * G : G;
+  int n, hk, grp, split;
+  grid.place((int)blockIdx.x, p, &n, &hk, &grp, &split);
+  const int h0 = hk * grid.share + grp * G, nh = grid.share - grp * G < G ? grid.share - grp * G : G;
   const KeyRange all = key_range(p, n), r = split_range(p, all, split);
   if (p.splits > 1 && split >= used_splits(p, all)) return;
 
@@ -203,32 +232,46 @@ __global__ void __launch_bounds__(512) paged_decode_rows(PagedDecodeParams p, Fa
   const unsigned keoff = ALIGNED ? (unsigned)(lr * p.c.ke2) : 0u, veoff = ALIGNED ? (unsigned)(lr * p.c.ve2) : 0u;
 
   // U steps of a wave, their loads ahead of their use: one batch is under way
-  // while the one before it is added up.
+  // while the one before it is added up, and the places of the next are looked
+  // up meanwhile.
+  struct Places {
+    int id[U], row[U];
+    bool ok[U];  // of this lane's row
+  };
   struct Batch {
     PK k[U];
     PV v[U];
     int ke[U], ve[U];
-    bool ok[U];  // of this lane's row
+    bool ok[U];
   };
-  auto load = [&](Batch& t, int64_t base) {
+  auto look = [&](int64_t base) {
+    Places w;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const unsigned pos = (unsigned)base + u * RPW + (ALIGNED ? 0 : lr), hi = (unsigned)r.hi;
       const int at = pos < hi ? (int)pos : r.hi - 1;
-      const int slot = fdiv(at, page_div);
-      int id = table[slot], row = at - slot * p.c.S;
-      t.ok[u] = id >= 0 && id < p.c.P;
-      id = t.ok[u] ? id : 0;
+      const int slot = fdiv(at, grid.page);
+      const int id = table[slot];
+      w.ok[u] = id >= 0 && id < p.c.P;
+      w.id[u] = w.ok[u] ? id : 0;
+      w.row[u] = at - slot * p.c.S;
       if (ALIGNED) {
-        row = pos < hi ? row : 0;  // a whole step past the end reads its page's first
-        t.ok[u] = t.ok[u] && pos + lr >= (unsigned)r.lo && pos + lr < hi;
+        w.row[u] = pos < hi ? w.row[u] : 0;  // a whole step past the end reads its page's first
+        w.ok[u] = w.ok[u] && pos + lr >= (unsigned)r.lo && pos + lr < hi;
       } else {
-        t.ok[u] = t.ok[u] && pos < hi;
+        w.ok[u] = w.ok[u] && pos < hi;
       }
-      t.k[u].load(kbase + (id * p.c.k.s0 + row * p.c.k.s2) * page_elt(KD), koff);
-      if constexpr (KE) t.ke[u] = (kebase + id * p.c.ke0 + row * p.c.ke2)[keoff];
-      t.v[u].load(vbase + (id * p.c.v.s0 + row * p.c.v.s2) * page_elt(VD), voff);
-      if constexpr (VE) t.ve[u] = (vebase + id * p.c.ve0 + row * p.c.ve2)[veoff];
+    }
+    return w;
+  };
+  auto load = [&](Batch& t, const Places& w) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      t.ok[u] = w.ok[u];
+      t.k[u].load(kbase + (w.id[u] * p.c.k.s0 + w.row[u] * p.c.k.s2) * page_elt(KD), koff);
+      if constexpr (KE) t.ke[u] = (kebase + w.id[u] * p.c.ke0 + w.row[u] * p.c.ke2)[keoff];
+      t.v[u].load(vbase + (w.id[u] * p.c.v.s0 + w.row[u] * p.c.v.s2) * page_elt(VD), voff);
+      if constexpr (VE) t.ve[u] = (vebase + w.id[u] * p.c.ve0 + w.row[u] * p.c.ve2)[veoff];
     }
   };
   auto add = [&](Batch& t) {
@@ -262,16 +305,19 @@ __global__ void __launch_bounds__(512) paged_decode_rows(PagedDecodeParams p, Fa
   int64_t base = (ALIGNED ? r.lo / RPW * RPW : r.lo) + (int64_t)wave * RPW * U;
   if (base < r.hi) {
     Batch t0, t1;
-    load(t0, base);
+    load(t0, look(base));
+    Places w = look(base + step);
     qraw.floats(p, ch, q);
     for (; base + 2 * step < r.hi; base += 2 * step) {
-      load(t1, base + step);
+      load(t1, w);
+      w = look(base + 2 * step);
       add(t0);
-      load(t0, base + 2 * step);
+      load(t0, w);
+      w = look(base + 3 * step);
       add(t1);
     }
     if (base + step < r.hi) {
-      load(t1, base + step);
+      load(t1, w);
       add(t0);
       add(t1);
     } else {
@@ -283,20 +329,22 @@ __global__ void __launch_bounds__(512) paged_decode_rows(PagedDecodeParams p, Fa
   const int D = p.D;
 #pragma unroll
   for (int g = 0; g < G; ++g) {
-    mass[g] = column_sum<LPR>(mass[g]);
+    using F = Fold<LPR, VPL>;
+    mass[g] = F::sum(mass[g]);
+    F::run(acc[g]);
+    float* o = red + (wave * G + g) * (D + 1);
+    if (F::write(lane)) {
 #pragma unroll
-    for (int e = 0; e < VPL; ++e) acc[g][e] = column_sum<LPR>(acc[g][e]);
-    if (lane < LPR) {
-      float* o = red + (wave * G + g) * (D + 1);
-#pragma unroll
-      for (int e = 0; e < VPL; ++e)
-        if (PV::feat(ch, e) < D) o[PV::feat(ch, e)] = acc[g][e];
-      if (lane == 0) o[D] = mass[g];
+      for (int j = 0; j < VPL / F::kParts; ++j) {
+        const int f = PV::feat(ch, F::kept(lane, j));
+        if (f < D) o[f] = acc[g][j];
+      }
     }
+    if (lane == 0) o[D] = mass[g];
   }
   __syncthreads();
   for (int i = tid; i < nh * D; i += (int)blockDim.x) {
-    const int g = i / D, d = i % D;
+    const int g = fdiv(i, grid.dim), d = i - g * D;
     float o = 0.f, m = 0.f;
     for (int w = 0; w < waves; ++w) {
       o += red[(w * G + g) * (D + 1) + d];
@@ -314,11 +362,10 @@ __global__ void __launch_bounds__(512) paged_decode_rows(PagedDecodeParams p, Fa
 
 template <int KD, int VD, int VPL, int LPR, int G, bool ALIGNED>
 void launch_rows_as(const PagedDecodeParams& p, int waves, hipStream_t st) {
-  constexpr int U = ALIGNED && G == 1 ? 2 : 1;
-  const int groups = (p.H / p.Hk + G - 1) / G;
+      constexpr int U = ALIGNED && G == 1 ? 2 : 1;
+  const DecodeGrid grid(p, G);
   paged_decode_rows<KD, VD, VPL, LPR, G, U, ALIGNED>
-      <<<(unsigned)((int64_t)p.N * p.Hk * groups * p.splits), 64 * waves, waves * G * (p.D + 1) * sizeof(float), st>>>(
-          p, fast_div(p.c.S));
+      <<<grid.size(p), 64 * waves, waves * G * (p.D + 1) * sizeof(float), st>>>(p, grid);
 }
 
 // Rows of pieces for this type, head dim, page size: the lanes of a row, the
