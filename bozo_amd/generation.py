@@ -187,20 +187,31 @@ class TensionKVCache:
         first = model.blocks[0].tension
         if first.rope_enabled:
             rot = (first.rope.cos.index_select(0, pos), first.rope.sin.index_select(0, pos))
-        fpos = None
+        fpos = _osc_positions(model, pos)
         for blk, c, par in zip(model.blocks, self.layers, parities):
             h = blk.pre_norm(x)
             h = _layer_step(blk.tension, h, c, par, rot, taus, self.return_all, t)
-            if blk.oscillate is not None:
-                osc = blk.oscillate
-                if fpos is None:
-                    fpos = osc.pos_buf.index_select(0, pos)
-                h = h * (1.0 + osc.amp * torch.sin(fpos * osc.freqs + osc.phases)[None])
-            ffn = blk.ffn
-            y = ffn.proj(torch.nn.functional.silu(ffn.gate(h)) * ffn.val(h))
-            # the residual in the stream's dtype (same values as x + y)
-            x = ffn.norm(h + y.to(h.dtype))
+            x = _after_tension(blk, h, fpos)
         return model.lm_head(model.final_norm(x))[:, 0]
+
+
+def _osc_positions(model, pos: Tensor) -> Optional[Tensor]:
+    """Positions pos [n] as the oscillatory modulation takes them, [n, 1],
+    gathered once for every block."""
+    osc = model.blocks[0].oscillate
+    return None if osc is None else osc.pos_buf.index_select(0, pos)
+
+
+def _after_tension(blk, h: Tensor, fpos: Optional[Tensor]) -> Tensor:
+    """The rest of a block behind its tension layer: h [N, T, D], modulated at
+    positions fpos [T, 1] (or [N, 1, 1]: each sequence's own), and the FFN."""
+    if blk.oscillate is not None:
+        osc = blk.oscillate
+        h = h * (1.0 + osc.amp * torch.sin(fpos * osc.freqs + osc.phases))
+    ffn = blk.ffn
+    y = ffn.proj(torch.nn.functional.silu(ffn.gate(h)) * ffn.val(h))
+    # the residual in the stream's dtype (same values as x + y)
+    return ffn.norm(h + y.to(h.dtype))
 
 
 def _layer_step(layer, x: Tensor, cache: TensionDecodeCache, par: int, rot, taus,
