@@ -20,6 +20,12 @@ inline FastDiv fast_div(int64_t d) {
   return {(unsigned)(((uint64_t)1 << 32) * (((uint64_t)1 << s) - d) / d + 1), s};
 }
 
+// Whether every row of b starts at a multiple of `bytes`.
+inline bool row_pieces(const Buf& b, int64_t bytes) {
+  const int64_t elt = b.dt == TENSION_E4M3 ? 1 : b.dt == TENSION_F32 ? 4 : 2;
+  return (uintptr_t)b.p % bytes == 0 && b.s0 * elt % bytes == 0 && b.s1 * elt % bytes == 0 && b.s2 * elt % bytes == 0;
+}
+
 struct KeyRange {
   int lo, hi;
 };

@@ -156,9 +156,9 @@ typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 struct Quads {
   int a, b;
 };
-template <bool F32, int LPR>
-__device__ __forceinline__ Quads lane_quads(int lane) {
-  return F32 ? Quads{4 * lane, 4 * LPR + 4 * lane} : Quads{8 * lane, 8 * lane + 4};
+template <bool F32>
+__device__ __forceinline__ Quads lane_quads(int lane, int D) {
+  return F32 ? Quads{4 * lane, D / 2 + 4 * lane} : Quads{8 * lane, 8 * lane + 4};
 }
 
 template <typename V>
@@ -201,6 +201,10 @@ struct Eight {
       *(u32x2*)((f16*)p + off + q.a) = u32x2{a[0][0], a[0][1]};
       *(u32x2*)((f16*)p + off + q.b) = u32x2{a[0][2], a[0][3]};
     }
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < (WIDE ? 2 : 1); ++i) a[i] = u32x4{0, 0, 0, 0};
   }
   __device__ __forceinline__ void floats(bool half, float* x) const {
     if constexpr (WIDE) {
@@ -247,38 +251,42 @@ struct Side {
   }
 
   __device__ __forceinline__ void load(const Buf& de, const Buf& pg, const uint8_t* ex, int64_t e0, int64_t e1, int64_t e2,
-                                       const Places<R>& w, int lane) {
-    const Quads q = lane_quads<F32, LPR>(lane);
+                                       const Places<R>& w, int lane, int D) {
+    const Quads q = lane_quads<F32>(lane, D);
+    const bool mine = 8 * lane < D;  // a lane past the head dim follows its row with zeros
     if constexpr (APPEND) {
       const int64_t off = w.n * de.s0 + w.t * de.s1 + w.h * de.s2;
 #pragma unroll
-      for (int r = 0; r < R; ++r)
-        if (w.live[r]) x[r].load(de, off + r * de.s1, q);
+      for (int r = 0; r < R; ++r) {
+        if (!mine) x[r].zero();
+        if (mine && w.live[r]) x[r].load(de, off + r * de.s1, q);
+      }
       return;
     }
     if (pg.dt == TENSION_E4M3) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const uint8_t* s = (const uint8_t*)pg.p + (w.live[r] ? page_off(pg, w, r) : 0);
+        const bool live = mine && w.live[r];
+        const uint8_t* s = (const uint8_t*)pg.p + (live ? page_off(pg, w, r) : 0);
         if constexpr (F32)
-          c[r] = u32x2{w.live[r] ? *(const unsigned*)(s + q.a) : 0, w.live[r] ? *(const unsigned*)(s + q.b) : 0};
+          c[r] = u32x2{live ? *(const unsigned*)(s + q.a) : 0, live ? *(const unsigned*)(s + q.b) : 0};
         else
-          c[r] = w.live[r] ? *(const u32x2*)(s + q.a) : u32x2{0, 0};
+          c[r] = live ? *(const u32x2*)(s + q.a) : u32x2{0, 0};
         b[r] = w.live[r] ? ex[w.id[r] * e0 + w.h * e1 + w.row[r] * e2] : 127;
       }
     } else if (pg.dt == de.dt) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const float zero[8] = {};
-        x[r].set(false, zero);
-        if (w.live[r]) x[r].load(pg, page_off(pg, w, r), q);
+        x[r].zero();
+        if (mine && w.live[r]) x[r].load(pg, page_off(pg, w, r), q);
       }
     }
   }
 
   __device__ __forceinline__ void store(const Buf& de, const Buf& pg, uint8_t* ex, int64_t e0, int64_t e1, int64_t e2,
-                                        const Places<R>& w, int lane) {
-    const Quads q = lane_quads<F32, LPR>(lane);
+                                        const Places<R>& w, int lane, int D) {
+    const Quads q = lane_quads<F32>(lane, D);
+    const bool mine = 8 * lane < D;  // a lane past the head dim follows its row with zeros
     const bool half = de.dt == TENSION_F16;
     if constexpr (APPEND) {
 #pragma unroll
@@ -286,7 +294,7 @@ struct Side {
         if (!w.live[r]) continue;  // a row's lanes agree
         const int64_t off = page_off(pg, w, r);
         if (pg.dt == de.dt) {
-          x[r].store(pg, off, q);
+          if (mine) x[r].store(pg, off, q);
           continue;
         }
         float f[8];
@@ -294,7 +302,7 @@ struct Side {
         if (pg.dt != TENSION_E4M3) {  // float32 tokens, 16-bit pages
           Eight<false> y;
           y.set(pg.dt == TENSION_F16, f);
-          y.store(pg, off, q);
+          if (mine) y.store(pg, off, q);
           continue;
         }
         unsigned top = 0;
@@ -310,9 +318,11 @@ struct Side {
         const u32x2 codes = {pack4(f[0], f[1], f[2], f[3]), pack4(f[4], f[5], f[6], f[7])};
         uint8_t* to = (uint8_t*)pg.p + off;
         if constexpr (F32) {
-          *(unsigned*)(to + q.a) = codes[0];
-          *(unsigned*)(to + q.b) = codes[1];
-        } else {
+          if (mine) {
+            *(unsigned*)(to + q.a) = codes[0];
+            *(unsigned*)(to + q.b) = codes[1];
+          }
+        } else if (mine) {
           *(u32x2*)(to + q.a) = codes;
         }
         if (lane == 0) ex[w.id[r] * e0 + w.h * e1 + w.row[r] * e2] = (uint8_t)e;
@@ -322,7 +332,7 @@ struct Side {
     const int64_t off = w.n * de.s0 + w.t * de.s1 + w.h * de.s2;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      if (!w.in[r]) continue;
+      if (!mine || !w.in[r]) continue;
       if (pg.dt == TENSION_E4M3) {
         float f[8];
         const float s = pow2_of_byte(b[r]);
@@ -388,17 +398,14 @@ __global__ void __launch_bounds__(kThreads) paged_rows_vec(PagedRowsParams p, Ve
   Side<APPEND, LPR, R, KF32> k;
   Side<APPEND, LPR, R, VF32> v;
   uint8_t *ke = const_cast<uint8_t*>(p.c.ke), *ve = const_cast<uint8_t*>(p.c.ve);
-  k.load(p.kd, p.c.k, ke, p.c.ke0, p.c.ke1, p.c.ke2, w, lane);
-  v.load(p.vd, p.c.v, ve, p.c.ve0, p.c.ve1, p.c.ve2, w, lane);
-  k.store(p.kd, p.c.k, ke, p.c.ke0, p.c.ke1, p.c.ke2, w, lane);
-  v.store(p.vd, p.c.v, ve, p.c.ve0, p.c.ve1, p.c.ve2, w, lane);
+  k.load(p.kd, p.c.k, ke, p.c.ke0, p.c.ke1, p.c.ke2, w, lane, p.D);
+  v.load(p.vd, p.c.v, ve, p.c.ve0, p.c.ve1, p.c.ve2, w, lane, p.D);
+  k.store(p.kd, p.c.k, ke, p.c.ke0, p.c.ke1, p.c.ke2, w, lane, p.D);
+  v.store(p.vd, p.c.v, ve, p.c.ve0, p.c.ve1, p.c.ve2, w, lane, p.D);
 }
 
-// Pieces of 8 values of a row are whole 16-byte (8-byte: e4m3) pieces of memory.
-bool vec_aligned(const Buf& b) {
-  const int64_t bytes = b.dt == TENSION_E4M3 ? 1 : b.dt == TENSION_F32 ? 4 : 2, to = b.dt == TENSION_E4M3 ? 8 : 16;
-  return (uintptr_t)b.p % to == 0 && b.s0 * bytes % to == 0 && b.s1 * bytes % to == 0 && b.s2 * bytes % to == 0;
-}
+// Pieces of 8 values of a row are whole pieces of memory.
+bool vec_aligned(const Buf& b) { return row_pieces(b, b.dt == TENSION_E4M3 ? 8 : 16); }
 
 template <bool APPEND, int R, bool KF32, bool VF32>
 bool launch_vec(const PagedRowsParams& p, hipStream_t st) {
@@ -416,13 +423,10 @@ bool launch_vec(const PagedRowsParams& p, hipStream_t st) {
     paged_rows_vec<APPEND, LPR, R, KF32, VF32><<<(unsigned)((g.units + per - 1) / per), kThreads, 0, st>>>(p, g);
     return true;
   };
-  switch (p.D) {
-    case 32: return go(std::integral_constant<int, 4>{});
-    case 64: return go(std::integral_constant<int, 8>{});
-    case 128: return go(std::integral_constant<int, 16>{});
-    case 256: return go(std::integral_constant<int, 32>{});
-    default: return false;
-  }
+  if (p.D <= 32) return go(std::integral_constant<int, 4>{});
+  if (p.D <= 64) return go(std::integral_constant<int, 8>{});
+  if (p.D <= 128) return go(std::integral_constant<int, 16>{});
+  return go(std::integral_constant<int, 32>{});
 }
 
 template <bool APPEND, int R>
@@ -432,8 +436,9 @@ bool launch_types(const PagedRowsParams& p, hipStream_t st) {
   return v ? launch_vec<APPEND, R, false, true>(p, st) : launch_vec<APPEND, R, false, false>(p, st);
 }
 
-// Head dims 32 to 256 (powers of two) with aligned rows.
+// Head dims in eights up to 256 with aligned rows.
 bool try_vec(bool append, const PagedRowsParams& p, hipStream_t st) {
+  if (p.D % 8 || p.D > 256) return false;
   if (!vec_aligned(p.kd) || !vec_aligned(p.vd) || !vec_aligned(p.c.k) || !vec_aligned(p.c.v)) return false;
   const int64_t threads = mul_cap((int64_t)p.N * p.T, (int64_t)p.Hk * p.D / 8, (int64_t)1 << 40);
   // Two tokens to a thread for reads that fill the card more than once (E4M3 to bf16, N8 Hk16 D64: T1024 12.6 -> 10.4

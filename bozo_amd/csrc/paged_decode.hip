@@ -120,25 +120,28 @@ void launch_join(const PagedDecodeParams& p, hipStream_t st) {
 
 }  // namespace
 
-// Splits of a sequence's keys.  A CU streams about 25 KB/us of cache whether
-// one workgroup or four run on it, so a call takes as long as its fullest CU;
-// the partial sums and the second kernel cost about 3 us more.  Tried: one
-// split, and what fills the CUs one to four times (two where the matrix kernel
+// Splits of a sequence's keys.  A CU by itself streams 49 KB/us of cache, all
+// of them 23 KB/us each; partial sums and the second kernel cost about 3 us
+// (bf16 D64, us for 1 / 21 splits: N1 H12 L512 6.3 / 7.2, L1024 9.2 / 7.3, L8192
+// 47 / 10; N16 H12, 1 / 5: L1000 10.2 / 12.3, L3000 25 / 28).  Tried: one split,
+// and what gives each CU one to four workgroups (two where the matrix kernel
 // holds head dim 128), with 128 keys to a split at least.
 void paged_decode_split(int64_t N, int64_t H, int64_t Hk, int64_t D, int64_t keys, int* splits, int* chunk) {
-  constexpr float kBytesPerUs = 25e3f, kJoinUs = 3.f;
+  constexpr float kCuBytesPerUs = 49e3f, kAllBytesPerUs = 23e3f, kJoinUs = 3.f;
   constexpr int64_t kLeast = 128;
   const int64_t rows = N * Hk, cus = device_cus();
-  const float row_us = (float)keys * (float)(4 * D) / kBytesPerUs;
+  const float row_bytes = (float)keys * (float)(4 * D);
+  const float all_us = (float)rows * row_bytes / (kAllBytesPerUs * (float)cus);
   const int fills = H > Hk && D > 64 ? 2 : 4;
-  float best = (float)((rows + cus - 1) / cus) * row_us;
+  float best = 0.f;
   int64_t ns = 1;
-  for (int f = 1; f <= fills; ++f) {
-    int64_t s = rows > 0 ? f * cus / rows : 1;
+  for (int f = 0; f <= fills; ++f) {
+    int64_t s = f == 0 || rows <= 0 ? 1 : f * cus / rows;
     s = s < keys / kLeast ? s : keys / kLeast;
-    if (s <= ns) continue;
-    const float t = (float)((rows * s + cus - 1) / cus) / (float)s * row_us + kJoinUs;
-    if (t < best) {
+    if (f > 0 && s <= ns) continue;
+    const float cu_us = (float)((rows * s + cus - 1) / cus) * row_bytes / (float)(s > 0 ? s : 1) / kCuBytesPerUs;
+    const float t = (cu_us > all_us ? cu_us : all_us) + (f > 0 ? kJoinUs : 0.f);
+    if (f == 0 || t < best) {
       best = t;
       ns = s;
     }

@@ -12,7 +12,7 @@
 //
 // Roundings: K, q and V enter as they are (an e4m3 code is a bf16 and an f16
 // number; its row's scale is applied to the score, or to tau).  tau enters as
-// two bf16 terms, off by 2^-17 of itself at most; sums are float32.
+// two bf16 terms, off by 2^-16 of itself at most; sums are float32.
 //
 // Bound by HBM: 32 keys of 128 e4m3 values (8.3 KB) take a wave about 900 cycles
 // of vector instructions, a quarter of what the card's rate leaves it; the time
@@ -199,14 +199,17 @@ __global__ void __launch_bounds__(64 * kWaves, F8 || D == 64 ? 3 : 2) paged_deco
       u32x4 th, tl;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        bf16x2 hi2, lo2;
+        // the first term is less than tau and the second positive: an infinite value row stays infinite
+        unsigned hi2 = 0;
+        bf16x2 lo2;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const float x = tau[j / 2][2 * (j % 2) + e];
-          hi2[e] = (bf16)x;
-          lo2[e] = (bf16)(x - (float)hi2[e]);
+          const unsigned w = x == 0.f ? 0u : (__builtin_bit_cast(unsigned, x) - 1) & 0xffff0000u;
+          hi2 |= e ? w : w >> 16;
+          lo2[e] = (bf16)(x - __builtin_bit_cast(float, w));
         }
-        th[j] = __builtin_bit_cast(unsigned, hi2);
+        th[j] = hi2;
         tl[j] = __builtin_bit_cast(unsigned, lo2);
       }
       if (!whole) {
@@ -295,6 +298,7 @@ bool launch_paged_decode_mfma(const PagedDecodeParams& p, hipStream_t st) {
   const bool f8 = p.c.k.dt == TENSION_E4M3;
   if ((p.D != 64 && p.D != 128) || p.c.S % kTileKeys || p.c.v.dt != p.c.k.dt) return false;
   if (f8 ? p.q.dt == TENSION_F32 : p.q.dt != TENSION_BF16 || p.c.k.dt != TENSION_BF16) return false;
+  if (!row_pieces(p.c.k, 16) || !row_pieces(p.c.v, 16)) return false;
   if ((uintptr_t)p.q.p % 16 || p.q.s0 % 8 || p.q.s1 % 8) return false;
   if (f8) {  // exponents of four rows are one word
     const uintptr_t a = (uintptr_t)p.c.ke | (uintptr_t)p.c.ke0 | (uintptr_t)p.c.ke1;
