@@ -74,7 +74,19 @@ __device__ __forceinline__ float pow2_of_byte(int b) { return __builtin_bit_cast
 struct DecodeGrid {
   FastDiv page, dim, splits, heads, group_div;
   int share, groups;  // query heads of a key head, and their groups
+  // Element strides of pages and rows, and whether values (exponents) lie as
+  // keys do: a step's place is a few scalar instructions, which a short step
+  // waits for as it does for its vector ones.
+  uint32_t k0, k2, v0, v2, ke0, ke2, ve0, ve2;
+  bool same, same_exp;
 
+  // Whether the strides are ones that the kernels take.
+  static bool fits(const PagedDecodeParams& p) {
+    auto ok = [&](int64_t page, int64_t row) {
+      return page >= 0 && page < ((int64_t)1 << 31) && row >= 0 && row < (1 << 24) && row * p.c.S < ((int64_t)1 << 31);
+    };
+    return ok(p.c.k.s0, p.c.k.s2) && ok(p.c.v.s0, p.c.v.s2) && ok(p.c.ke0, p.c.ke2) && ok(p.c.ve0, p.c.ve2);
+  }
   DecodeGrid(const PagedDecodeParams& p, int per_group) {
     share = p.H / p.Hk;
     groups = (share + per_group - 1) / per_group;
@@ -83,6 +95,26 @@ struct DecodeGrid {
     splits = fast_div(p.splits);
     heads = fast_div(p.Hk);
     group_div = fast_div(groups);
+    k0 = (uint32_t)p.c.k.s0, k2 = (uint32_t)p.c.k.s2, v0 = (uint32_t)p.c.v.s0, v2 = (uint32_t)p.c.v.s2;
+    ke0 = (uint32_t)p.c.ke0, ke2 = (uint32_t)p.c.ke2, ve0 = (uint32_t)p.c.ve0, ve2 = (uint32_t)p.c.ve2;
+    same = k0 == v0 && k2 == v2;
+    same_exp = ke0 == ve0 && ke2 == ve2;
+  }
+  // Elements from the first page's first row to this one's, of a head.
+  struct Place {
+    uint64_t k, v, ke, ve;
+  };
+  template <bool EXP>
+  __device__ __forceinline__ Place at(int id, int row) const {
+    auto off = [&](uint32_t s0, uint32_t s2) { return (uint64_t)(uint32_t)id * s0 + (uint32_t)row * s2; };
+    Place w{};
+    w.k = off(k0, k2);
+    w.v = same ? w.k : off(v0, v2);
+    if constexpr (EXP) {
+      w.ke = off(ke0, ke2);
+      w.ve = same_exp ? w.ke : off(ve0, ve2);
+    }
+    return w;
   }
   unsigned size(const PagedDecodeParams& p) const { return (unsigned)((int64_t)p.N * p.Hk * groups * p.splits); }
   __device__ __forceinline__ void place(int b, const PagedDecodeParams& p, int* n, int* hk, int* grp, int* split) const {

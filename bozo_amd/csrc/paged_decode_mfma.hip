@@ -100,24 +100,26 @@ __global__ void __launch_bounds__(64 * kWaves, F8 || D == 64 ? 3 : 2) paged_deco
     page_ok[t] = x >= 0 && x < p.c.P;
     *id = page_ok[t] ? x : 0;
   };
-  int id[2], row[2];
+  DecodeGrid::Place at[2];
   auto load_k = [&](int64_t base) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      where(base, t, &id[t], &row[t]);
-      const char* s = kbase + (id[t] * p.c.k.s0 + row[t] * p.c.k.s2) * kElt;
+      int id, row;
+      where(base, t, &id, &row);
+      at[t] = grid.at<F8>(id, row);
+      const char* s = kbase + at[t].k * kElt;
 #pragma unroll
       for (int i = 0; i < KP; ++i) kr[t][i] = __builtin_nontemporal_load((const u32x4*)(s + koff + 64 * i));
       if constexpr (F8) {
-        ke[t] = *(const unsigned*)(kebase + id[t] * p.c.ke0 + row[t] + 4 * g);
-        ve[t] = *(const unsigned*)(vebase + id[t] * p.c.ve0 + row[t] + 4 * g);
+        ke[t] = *(const unsigned*)(kebase + at[t].ke + 4 * g);
+        ve[t] = *(const unsigned*)(vebase + at[t].ve + 4 * g);
       }
     }
   };
   auto load_v = [&]() {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const char* s = vbase + (id[t] * p.c.v.s0 + row[t] * p.c.v.s2) * kElt;
+      const char* s = vbase + at[t].v * kElt;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         typedef unsigned piece __attribute__((ext_vector_type(VW)));

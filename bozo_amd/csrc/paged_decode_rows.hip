@@ -11,11 +11,8 @@ bool launch_paged_rows_e4m3(const PagedDecodeParams&, int waves, hipStream_t);
 
 namespace {
 
-// Pieces of 8 values are whole pieces of memory, and a wave's rows of a step
-// span 32 bits.
-bool rows_aligned(const Buf& b) {
-  return row_pieces(b, b.dt == TENSION_E4M3 ? 8 : 16) && b.s2 >= 0 && b.s2 < (1 << 24);
-}
+// Pieces of 8 values are whole pieces of memory.
+bool rows_aligned(const Buf& b) { return row_pieces(b, b.dt == TENSION_E4M3 ? 8 : 16); }
 
 // Waves of a workgroup.  Up to one workgroup per CU the call waits for memory
 // (N16 H12, 1000 bf16 keys: eight waves 10.2 us, four 12.3), and where each
@@ -34,7 +31,7 @@ int waves_for(const PagedDecodeParams& p) {
 
 bool launch_paged_decode_rows(const PagedDecodeParams& p, hipStream_t st) {
   if (p.D % 8 || !rows_aligned(p.c.k) || !rows_aligned(p.c.v)) return false;
-  if (p.c.ke2 < 0 || p.c.ke2 >= (1 << 24) || p.c.ve2 < 0 || p.c.ve2 >= (1 << 24)) return false;
+  if (!DecodeGrid::fits(p)) return false;
   // A shared key head on the matrix units where its types allow: two query heads cost the same either way (bf16 D64,
   // 268 MB: 48 us), four 48.8 against 59.0 us, eight 50 against 102; e4m3 D128, 135 MB, four heads 30 against 50 us.
   if (p.H / p.Hk >= 2 && launch_paged_decode_mfma(p, st)) return true;

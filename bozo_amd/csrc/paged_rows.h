@@ -268,10 +268,11 @@ __global__ void __launch_bounds__(G == 1 ? 1024 : 512) paged_decode_rows(PagedDe
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       t.ok[u] = w.ok[u];
-      t.k[u].load(kbase + (w.id[u] * p.c.k.s0 + w.row[u] * p.c.k.s2) * page_elt(KD), koff);
-      if constexpr (KE) t.ke[u] = (kebase + w.id[u] * p.c.ke0 + w.row[u] * p.c.ke2)[keoff];
-      t.v[u].load(vbase + (w.id[u] * p.c.v.s0 + w.row[u] * p.c.v.s2) * page_elt(VD), voff);
-      if constexpr (VE) t.ve[u] = (vebase + w.id[u] * p.c.ve0 + w.row[u] * p.c.ve2)[veoff];
+      const DecodeGrid::Place at = grid.at<KE>(w.id[u], w.row[u]);
+      t.k[u].load(kbase + at.k * page_elt(KD), koff);
+      if constexpr (KE) t.ke[u] = (kebase + at.ke)[keoff];
+      t.v[u].load(vbase + at.v * page_elt(VD), voff);
+      if constexpr (VE) t.ve[u] = (vebase + at.ve)[veoff];
     }
   };
   auto add = [&](Batch& t) {

@@ -176,7 +176,9 @@ def paged_decode(q: Tensor, kv: PagedKV, table: Tensor, lengths: Tensor, scale: 
     range) or None / "raw", as in ``decode_step``.  H may be a multiple of the
     pages' heads: query head h reads key head h // (H / Hk).  max_len: a bound
     of the lengths known on the host, by which the launch is shaped (default:
-    what the table can hold); it does not cut a longer sequence.  Returns out
+    what the table can hold); it does not cut a longer sequence.  Sequences
+    start in their order: where lengths differ much, longest first is faster
+    (N64 H12, 500 to 2048 e4m3 tokens: 26 us against 29).  Returns out
     [N, H, D] in q.dtype, zeros for a sequence with no key."""
     flags = _DECODE_NORMS.get(normalize)
     W = 0 if window is None else int(window)
