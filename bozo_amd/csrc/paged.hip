@@ -1,6 +1,8 @@
 // Paged K/V cache: tokens written into pages (quantised to e4m3 on the way or
 // as they are) and read back dense.  Both are streams: a row of D values is
-// read once and written once, so HBM bounds them.
+// read once and written once, so HBM bounds them (bf16 prompts, 262 MB: 52 us,
+// 5.0 TB/s, what a large copy reaches; e4m3 read back, 303 MB: 62 to 67 us), and
+// below some 20 MB the chain of start, table, rows (about 4 us).
 //
 // Quantised rows: with E the biased exponent of a row's largest finite
 // magnitude a and M its mantissa bits, 448 = 1.75 * 2^8 gives the smallest e
@@ -367,7 +369,8 @@ struct Side {
 
 // LPR lanes to a row, R tokens of one head to a thread, K and V both.
 // Consecutive units are heads of one token, so a wave's rows lie together in
-// the dense tensors, and a thread's tokens lie together in a page.
+// the dense tensors, and a thread's tokens lie together in a page.  (Tokens of
+// one head side by side, K and V apart: prompts 73.5 us for 52, read 123 for 62.)
 template <bool APPEND, int LPR, int R, bool KF32, bool VF32>
 __global__ void __launch_bounds__(kThreads) paged_rows_vec(PagedRowsParams p, VecGeometry g) {
   const int lane = threadIdx.x % LPR;

@@ -10,63 +10,96 @@ namespace tension {
 
 namespace {
 
-constexpr int kThreads = 256;
-
-__device__ __forceinline__ float ld_page(const Buf& b, int64_t off) {
-  return b.dt == TENSION_E4M3 ? __builtin_amdgcn_cvt_f32_fp8((int)((const uint8_t*)b.p)[off], 0) : ld<float>(b, off);
-}
-
 // ------------------------------------------------------------------ any types, head dim <= 256, any page size
 
-// One workgroup per (n, h, split): a thread forms the tau of one key, then
-// threads along the head dim add the value rows.
-__global__ void __launch_bounds__(kThreads) paged_decode_any(PagedDecodeParams p) {
-  __shared__ float qs[256], tau[kThreads], red[kThreads / 64];
-  __shared__ int64_t voff[kThreads];
-  const int tid = threadIdx.x;
+// Values ch, ch + 16, ... of a row as their bits, and as floats.
+template <int VPL>
+__device__ __forceinline__ void load_bits(const Buf& b, int64_t row, int ch, int D, unsigned* w) {
+#pragma unroll
+  for (int e = 0; e < VPL; ++e) w[e] = 0;
+  auto go = [&](auto* s) {
+#pragma unroll
+    for (int e = 0; e < VPL; ++e)
+      if (ch + 16 * e < D) w[e] = s[row + ch + 16 * e];
+  };
+  if (b.dt == TENSION_F32) go((const uint32_t*)b.p);
+  else if (b.dt == TENSION_E4M3) go((const uint8_t*)b.p);
+  else go((const uint16_t*)b.p);
+}
+template <int VPL>
+__device__ __forceinline__ void bits_to_floats(int dt, const unsigned* w, float* x) {
+#pragma unroll
+  for (int e = 0; e < VPL; ++e) {
+    if (dt == TENSION_F32) x[e] = __builtin_bit_cast(float, w[e]);
+    else if (dt == TENSION_BF16) x[e] = __builtin_bit_cast(float, w[e] << 16);
+    else if (dt == TENSION_F16) x[e] = (float)__builtin_bit_cast(f16, (unsigned short)w[e]);
+    else x[e] = __builtin_amdgcn_cvt_f32_fp8((int)w[e], 0);
+  }
+}
+
+// One workgroup per (n, h, split), sixteen lanes to a row, a value at a time:
+// for rows that are no whole pieces of eight values, and pairs of types that
+// have no kernel of their own.  Bound by its loads' number and latency (N16 H12,
+// 1000 keys: bf16 D20 30 us, D100 127; D24 on the kernels for whole pieces 6.2).
+template <int VPL, int kWaves>
+__global__ void __launch_bounds__(64 * kWaves) paged_decode_any(PagedDecodeParams p) {
+  constexpr int kRows = 4;
+  __shared__ float red[kWaves][16 * VPL + 1];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, ch = lane & 15;
   const int i = blockIdx.x % p.splits, nh = blockIdx.x / p.splits;
   const int n = nh / p.H, h = nh % p.H, hk = h / (p.H / p.Hk);
   const KeyRange all = key_range(p, n), r = split_range(p, all, i);
   if (p.splits > 1 && i >= used_splits(p, all)) return;
-  for (int d = tid; d < p.D; d += kThreads) qs[d] = ld<float>(p.q, n * p.q.s0 + h * p.q.s1 + d);
-  __syncthreads();
-  float acc = 0.f, mass = 0.f;
-  for (int base = r.lo; base < r.hi; base += kThreads) {
-    const int m = r.hi - base < kThreads ? r.hi - base : kThreads;
-    float w = 0.f;
-    int64_t vo = -1;
-    if (tid < m) {
-      const int pos = base + tid, row = pos % p.c.S;
-      const int page = p.c.table[(int64_t)n * p.c.table_stride + pos / p.c.S];
-      if (page >= 0 && page < p.c.P) {
-        const int64_t ko = page * p.c.k.s0 + hk * p.c.k.s1 + row * p.c.k.s2;
-        float s = 0.f;
-        for (int d = 0; d < p.D; ++d) s += qs[d] * ld_page(p.c.k, ko + d);
-        if (p.c.ke) s *= pow2_of_byte(p.c.ke[page * p.c.ke0 + hk * p.c.ke1 + row * p.c.ke2]);
-        w = sigmoid_exact(s / p.scale);
-        mass += w;
-        if (p.c.ve) w *= pow2_of_byte(p.c.ve[page * p.c.ve0 + hk * p.c.ve1 + row * p.c.ve2]);
-        vo = page * p.c.v.s0 + hk * p.c.v.s1 + row * p.c.v.s2;
-      }
-    }
-    tau[tid] = w;
-    voff[tid] = vo;
-    __syncthreads();
-    if (tid < p.D)
-      for (int j = 0; j < m; ++j)
-        if (voff[j] >= 0) acc += tau[j] * ld_page(p.c.v, voff[j] + tid);
-    __syncthreads();
+  unsigned kw[VPL], vw[VPL];
+  float q[VPL], acc[VPL], x[VPL], mass = 0.f;
+  load_bits<VPL>(p.q, n * p.q.s0 + h * p.q.s1, ch, p.D, kw);
+  bits_to_floats<VPL>(p.q.dt, kw, q);
+#pragma unroll
+  for (int e = 0; e < VPL; ++e) acc[e] = 0.f;
+  for (int64_t base = (int64_t)r.lo + wave * kRows + (lane >> 4); base < r.hi; base += kWaves * kRows) {
+    const int pos = (int)base, row = pos % p.c.S;
+    const int page = p.c.table[(int64_t)n * p.c.table_stride + pos / p.c.S];
+    if (page < 0 || page >= p.c.P) continue;  // the sixteen lanes of a row agree
+    load_bits<VPL>(p.c.k, page * p.c.k.s0 + hk * p.c.k.s1 + row * p.c.k.s2, ch, p.D, kw);
+    load_bits<VPL>(p.c.v, page * p.c.v.s0 + hk * p.c.v.s1 + row * p.c.v.s2, ch, p.D, vw);
+    float s = 0.f, f = 1.f;
+    if (p.c.ve) f = pow2_of_byte(p.c.ve[page * p.c.ve0 + hk * p.c.ve1 + row * p.c.ve2]);
+    bits_to_floats<VPL>(p.c.k.dt, kw, x);
+#pragma unroll
+    for (int e = 0; e < VPL; ++e) s += q[e] * x[e];
+    s += dpp_move<0xB1>(s);   // lane ^ 1
+    s += dpp_move<0x4E>(s);   // lane ^ 2
+    s += dpp_move<0x141>(s);  // mirrored halves of 8
+    s += dpp_move<0x140>(s);  // mirrored rows of 16
+    if (p.c.ke) s *= pow2_of_byte(p.c.ke[page * p.c.ke0 + hk * p.c.ke1 + row * p.c.ke2]);
+    const float tau = sigmoid_exact(s / p.scale);
+    mass += tau;
+    bits_to_floats<VPL>(p.c.v.dt, vw, x);
+#pragma unroll
+    for (int e = 0; e < VPL; ++e) acc[e] += tau * f * x[e];
   }
 #pragma unroll
-  for (int m = 32; m; m >>= 1) mass += __shfl_xor(mass, m);
-  if ((tid & 63) == 0) red[tid >> 6] = mass;
+  for (int e = 0; e < VPL; ++e) {
+    acc[e] += __shfl_xor(acc[e], 16);
+    acc[e] += __shfl_xor(acc[e], 32);
+    if (lane < 16) red[wave][ch + 16 * e] = acc[e];
+  }
+  mass += __shfl_xor(mass, 16);
+  mass += __shfl_xor(mass, 32);
+  if (lane == 0) red[wave][16 * VPL] = mass;
   __syncthreads();
-  mass = red[0] + red[1] + red[2] + red[3];
+  if (tid >= p.D) return;
+  float o = 0.f, m = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    o += red[w][tid];
+    m += red[w][16 * VPL];
+  }
   if (p.splits > 1) {
-    if (tid < p.D) split_sums(p, nh, i)[tid] = acc;
-    if (tid == 0) *split_mass(p, nh, i) = mass;
-  } else if (tid < p.D) {
-    st<float>(p.out, n * p.out.s0 + h * p.out.s1 + tid, acc * norm_factor(p, mass, all));
+    split_sums(p, nh, i)[tid] = o;
+    if (tid == 0) *split_mass(p, nh, i) = m;
+  } else {
+    st<float>(p.out, n * p.out.s0 + h * p.out.s1 + tid, o * norm_factor(p, m, all));
   }
 }
 
@@ -121,23 +154,25 @@ void launch_join(const PagedDecodeParams& p, hipStream_t st) {
 }  // namespace
 
 // Splits of a sequence's keys.  A CU by itself streams 49 KB/us of cache, all
-// of them 23 KB/us each; partial sums and the second kernel cost about 3 us
-// (bf16 D64, us for 1 / 21 splits: N1 H12 L512 6.3 / 7.2, L1024 9.2 / 7.3, L8192
-// 47 / 10; N16 H12, 1 / 5: L1000 10.2 / 12.3, L3000 25 / 28).  Tried: one split,
-// and what gives each CU one to four workgroups (two where the matrix kernel
-// holds head dim 128), with 128 keys to a split at least.
+// of them 23 KB/us each; partial sums and the second kernel cost about 3 us on
+// the card, 4 on the host (bf16 D64, us in one kernel / split: N1 H12 L512 5.5 /
+// 7.2, L1024 9.2 / 7.1, L8192 47 / 10; N16 H12 L1000 10.1 / 12.3, L3000 25 / 28).
+// Tried: one split, and what gives each CU one to four workgroups (two where
+// the matrix kernel holds head dim 128), with 128 keys to a split at least.
 void paged_decode_split(int64_t N, int64_t H, int64_t Hk, int64_t D, int64_t keys, int* splits, int* chunk) {
-  constexpr float kCuBytesPerUs = 49e3f, kAllBytesPerUs = 23e3f, kJoinUs = 3.f;
+  constexpr float kCuBytesPerUs = 49e3f, kAllBytesPerUs = 23e3f, kJoinUs = 3.5f;
   constexpr int64_t kLeast = 128;
   const int64_t rows = N * Hk, cus = device_cus();
   const float row_bytes = (float)keys * (float)(4 * D);
   const float all_us = (float)rows * row_bytes / (kAllBytesPerUs * (float)cus);
   const int fills = H > Hk && D > 64 ? 2 : 4;
+  int64_t most = keys / kLeast;
+  if (N * H > 0 && most > ((int64_t)1 << 30) / (N * H)) most = ((int64_t)1 << 30) / (N * H);  // workgroups of a launch
   float best = 0.f;
   int64_t ns = 1;
   for (int f = 0; f <= fills; ++f) {
     int64_t s = f == 0 || rows <= 0 ? 1 : f * cus / rows;
-    s = s < keys / kLeast ? s : keys / kLeast;
+    s = s < most ? s : most;
     if (f > 0 && s <= ns) continue;
     const float cu_us = (float)((rows * s + cus - 1) / cus) * row_bytes / (float)(s > 0 ? s : 1) / kCuBytesPerUs;
     const float t = (cu_us > all_us ? cu_us : all_us) + (f > 0 ? kJoinUs : 0.f);
@@ -157,8 +192,11 @@ void paged_decode_split(int64_t N, int64_t H, int64_t Hk, int64_t D, int64_t key
 }
 
 int launch_paged_decode(const PagedDecodeParams& p, hipStream_t st, hipError_t* err) {
-  if (!launch_paged_decode_rows(p, st))
-    paged_decode_any<<<(unsigned)((int64_t)p.N * p.H * p.splits), kThreads, 0, st>>>(p);
+  if (!launch_paged_decode_rows(p, st)) {
+    const unsigned grid = (unsigned)((int64_t)p.N * p.H * p.splits);
+    if (p.D <= 64) paged_decode_any<4, 16><<<grid, 1024, 0, st>>>(p);
+    else paged_decode_any<16, 8><<<grid, 512, 0, st>>>(p);
+  }
   *err = hipGetLastError();
   if (*err == hipSuccess && p.splits > 1) {
     if (p.D <= 64) launch_join<64>(p, st);

@@ -16,10 +16,11 @@
 //
 // Bound by HBM: 32 keys of 128 e4m3 values (8.3 KB) take a wave about 900 cycles
 // of vector instructions, a quarter of what the card's rate leaves it; the time
-// hardly grows with the heads (bf16 D64, 268 MB: two heads 48.1 us, eight 50.5,
-// 5.3-5.6 TB/s).  The next step's K and V are loaded as soon as this step's are
-// operands.  Three waves per SIMD for e4m3 at head dim 128 (152 registers); bf16
-// there keeps two (three spill: 90 -> 101 us).
+// hardly grows with the heads (bf16 D64, 268 MB, two to eight heads: 43.8 to
+// 46.1 us, 5.8-6.1 TB/s; e4m3 D128, N2, 65500 keys, 135 MB: 25.7 us, 5.3 TB/s).
+// The next step's K and V are loaded as soon as this step's are operands.
+// Three waves per SIMD for e4m3 at head dim 128 (152 registers); bf16 there
+// keeps two (three spill: 90 -> 101 us).
 #include "mfma_common.h"
 #include "paged.h"
 
