@@ -20,10 +20,12 @@ inline FastDiv fast_div(int64_t d) {
   return {(unsigned)(((uint64_t)1 << 32) * (((uint64_t)1 << s) - d) / d + 1), s};
 }
 
-// Whether every row of b starts at a multiple of `bytes`.
-inline bool row_pieces(const Buf& b, int64_t bytes) {
-  const int64_t elt = b.dt == TENSION_E4M3 ? 1 : b.dt == TENSION_F32 ? 4 : 2;
-  return (uintptr_t)b.p % bytes == 0 && b.s0 * elt % bytes == 0 && b.s1 * elt % bytes == 0 && b.s2 * elt % bytes == 0;
+// Whether every row of b starts at a multiple of `bytes`, a power of two (of
+// which a wrapped product keeps the remainder).
+inline bool row_pieces(const Buf& b, uint64_t bytes) {
+  const uint64_t elt = b.dt == TENSION_E4M3 ? 1 : b.dt == TENSION_F32 ? 4 : 2;
+  auto whole = [&](int64_t s) { return (uint64_t)s * elt % bytes == 0; };
+  return (uintptr_t)b.p % bytes == 0 && whole(b.s0) && whole(b.s1) && whole(b.s2);
 }
 
 struct KeyRange {
