@@ -192,6 +192,26 @@ def test_infinities_and_nan_stay_in_their_places(pages, q, share, D):
     assert int(torch.isinf(out).sum()) == 2 * share
 
 
+@pytest.mark.parametrize("pages,q,share", [("bf16", "bf16", 1), ("bf16", "bf16", 4), ("f32", "f32", 1), ("f32", "f32", 4),
+                                           ("f16", "f16", 2)])
+@pytest.mark.parametrize("D", [20, 40, 64, 72, 96, 128])
+def test_infinite_keys_saturate(pages, q, share, D):
+    """A key with an infinity has tau 0 or 1, by the sign of the query there."""
+    S, Hk, lengths = 16, 2, [40, 33, 20]
+    table, P = make_table(lengths, S, seed=29)
+    kv = fill(PagedKV.empty(P, S, Hk, D, DT[pages]), 31)
+    x = query(3, Hk * share, D, q)
+    clean = [values(kv.k, None), values(kv.v, None)]
+    _, keys, mag, dots = R.decode(np64(x), *clean, table, lengths, math.sqrt(D))
+    for n, pos, f in ((0, 7, 0), (1, 32, D - 1), (2, 0, 5)):
+        pg, rw = R.place(table, P, S, n, pos)
+        kv.k[pg, :, rw, f] = float("inf")
+    ref, keys, mag, _ = R.decode(np64(x), values(kv.k, None), clean[1], table, lengths, math.sqrt(D))
+    out = np64(run_decode(x, kv, table, lengths, math.sqrt(D)))
+    bound = R.decode_bound(ref, keys, mag, dots, D, torch.finfo(x.dtype).eps) + (2.0 ** -25 if q == "f16" else 0)
+    assert np.isfinite(out).all() and (np.abs(out - ref) <= bound).all()
+
+
 def test_nan_codes():
     """The e4m3 form of the same: infinities were stored as NaN."""
     S, lengths, D = 16, [40, 33], 64
