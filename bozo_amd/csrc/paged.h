@@ -76,11 +76,10 @@ __device__ __forceinline__ float pow2_of_byte(int b) { return __builtin_bit_cast
 struct DecodeGrid {
   FastDiv page, dim, splits, heads, group_div;
   int share, groups;  // query heads of a key head, and their groups
-  // Element strides of pages and rows, and whether values (exponents) lie as
-  // keys do: a step's place is a few scalar instructions, which a short step
-  // waits for as it does for its vector ones.
+  // Element strides of pages and rows: a step's place is a few scalar
+  // instructions, which a short step waits for as it does for its vector ones.
   uint32_t k0, k2, v0, v2, ke0, ke2, ve0, ve2;
-  bool same, same_exp;
+  bool alike;  // values and their exponents lie as keys and theirs do
 
   // Whether the strides are ones that the kernels take.
   static bool fits(const PagedDecodeParams& p) {
@@ -99,22 +98,23 @@ struct DecodeGrid {
     group_div = fast_div(groups);
     k0 = (uint32_t)p.c.k.s0, k2 = (uint32_t)p.c.k.s2, v0 = (uint32_t)p.c.v.s0, v2 = (uint32_t)p.c.v.s2;
     ke0 = (uint32_t)p.c.ke0, ke2 = (uint32_t)p.c.ke2, ve0 = (uint32_t)p.c.ve0, ve2 = (uint32_t)p.c.ve2;
-    same = k0 == v0 && k2 == v2;
-    same_exp = ke0 == ve0 && ke2 == ve2;
+    alike = k0 == v0 && k2 == v2 && ke0 == ve0 && ke2 == ve2;
   }
   // Elements from the first page's first row to this one's, of a head.
   struct Place {
     uint64_t k, v, ke, ve;
   };
-  template <bool EXP>
+  template <bool EXP, bool ALIKE>
   __device__ __forceinline__ Place at(int id, int row) const {
     auto off = [&](uint32_t s0, uint32_t s2) { return (uint64_t)(uint32_t)id * s0 + (uint32_t)row * s2; };
     Place w{};
     w.k = off(k0, k2);
-    w.v = same ? w.k : off(v0, v2);
-    if constexpr (EXP) {
-      w.ke = off(ke0, ke2);
-      w.ve = same_exp ? w.ke : off(ve0, ve2);
+    if constexpr (EXP) w.ke = off(ke0, ke2);
+    w.v = w.k;
+    w.ve = w.ke;
+    if (!ALIKE && !alike) {
+      w.v = off(v0, v2);
+      if constexpr (EXP) w.ve = off(ve0, ve2);
     }
     return w;
   }

@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(64 * kWaves, F8 || D == 64 ? 3 : 2) paged_deco
     for (int t = 0; t < 2; ++t) {
       int id, row;
       where(base, t, &id, &row);
-      at[t] = grid.at<F8>(id, row);
+      at[t] = grid.at<F8, false>(id, row);
       const char* s = kbase + at[t].k * kElt;
 #pragma unroll
       for (int i = 0; i < KP; ++i) kr[t][i] = __builtin_nontemporal_load((const u32x4*)(s + koff + 64 * i));

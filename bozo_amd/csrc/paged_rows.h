@@ -211,8 +211,9 @@ struct Query {
   }
 };
 
-// FULL: the head dim fills a row's lanes.
-template <int KD, int VD, int VPL, int LPR, int G, int U, bool ALIGNED, bool FULL>
+// PLAIN: the head dim fills a row's lanes, and values and their exponents lie as
+// keys and theirs do.
+template <int KD, int VD, int VPL, int LPR, int G, int U, bool ALIGNED, bool PLAIN>
 __global__ void __launch_bounds__(G == 1 ? 1024 : 512) paged_decode_rows(PagedDecodeParams p, DecodeGrid grid) {
   constexpr int RPW = 64 / LPR;
   constexpr bool KE = KD == TENSION_E4M3, VE = VD == TENSION_E4M3;
@@ -288,7 +289,7 @@ __global__ void __launch_bounds__(G == 1 ? 1024 : 512) paged_decode_rows(PagedDe
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       t.ok[u] = w.ok[u];
-      const DecodeGrid::Place at = grid.at<KE>(w.id[u], w.row[u]);
+      const DecodeGrid::Place at = grid.at<KE, PLAIN>(w.id[u], w.row[u]);
       t.k[u].load(kbase + at.k * page_elt(KD), koff);
       if constexpr (KE) t.ke[u] = (kebase + at.ke)[keoff];
       t.v[u].load(vbase + at.v * page_elt(VD), voff);
@@ -298,11 +299,10 @@ __global__ void __launch_bounds__(G == 1 ? 1024 : 512) paged_decode_rows(PagedDe
   auto add = [&](Batch& t) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (!__all(t.ok[u])) {  // rows out of range or without a page hold anything
-        t.v[u].zero_unless(t.ok[u]);
-        if constexpr (VE) t.ve[u] = t.ok[u] ? t.ve[u] : 0;
-      }
-      if (!FULL && p.D < LPR * VPL) t.k[u].past(ch, p.D);  // an infinite key times a query's zeros is no number
+      // rows out of range or without a page hold anything (a branch that most steps would skip costs more)
+      t.v[u].zero_unless(t.ok[u]);
+      if constexpr (VE) t.ve[u] = t.ok[u] ? t.ve[u] : 0;
+      if (!PLAIN && p.D < LPR * VPL) t.k[u].past(ch, p.D);  // an infinite key times a query's zeros is no number
       float x[VPL], tau[G];
       t.k[u].floats(x);
 #pragma unroll
@@ -389,7 +389,7 @@ void launch_rows_as(const PagedDecodeParams& p, int waves, hipStream_t st) {
   const DecodeGrid grid(p, G);
   const unsigned n = grid.size(p), threads = 64 * waves, lds = waves * G * (p.D + 1) * sizeof(float);
   if constexpr (kOne) {
-    if (p.D == LPR * VPL) {  // the zeros of the other form cost 5% of an e4m3 stream
+    if (p.D == LPR * VPL && grid.alike) {  // what the other form checks costs 5% and more of an e4m3 stream
       paged_decode_rows<KD, VD, VPL, LPR, G, U, ALIGNED, true><<<n, threads, lds, st>>>(p, grid);
       return;
     }
