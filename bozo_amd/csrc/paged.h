@@ -76,6 +76,7 @@ __device__ __forceinline__ float pow2_of_byte(int b) { return __builtin_bit_cast
 struct DecodeGrid {
   FastDiv page, dim, splits, heads, group_div;
   int share, groups;  // query heads of a key head, and their groups
+  int waves;          // of a workgroup
   // Element strides of pages and rows: a step's place is a few scalar
   // instructions, which a short step waits for as it does for its vector ones.
   uint32_t k0, k2, v0, v2, ke0, ke2, ve0, ve2;
@@ -88,7 +89,7 @@ struct DecodeGrid {
     };
     return ok(p.c.k.s0, p.c.k.s2) && ok(p.c.v.s0, p.c.v.s2) && ok(p.c.ke0, p.c.ke2) && ok(p.c.ve0, p.c.ve2);
   }
-  DecodeGrid(const PagedDecodeParams& p, int per_group) {
+  DecodeGrid(const PagedDecodeParams& p, int per_group, int waves_) : waves(waves_) {
     share = p.H / p.Hk;
     groups = (share + per_group - 1) / per_group;
     page = fast_div(p.c.S);

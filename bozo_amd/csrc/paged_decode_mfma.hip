@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(64 * kWaves, F8 || D == 64 ? 3 : 2) paged_deco
 
 template <bool F8, bool QF16>
 void launch_as(const PagedDecodeParams& p, hipStream_t st) {
-  const DecodeGrid grid(p, 16);
+  const DecodeGrid grid(p, 16, 0);
   const unsigned n = grid.size(p);
   // eight waves where a CU has one workgroup
   const bool eight = n <= (unsigned)device_cus();

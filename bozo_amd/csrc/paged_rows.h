@@ -221,12 +221,12 @@ __global__ void __launch_bounds__(G == 1 ? 1024 : 512) paged_decode_rows(PagedDe
   using PV = Piece<VD, VPL, LPR>;
   extern __shared__ float red[];  // [waves][G][D + 1]
   const int tid = threadIdx.x, lane = tid & 63, ch = lane % LPR, lr = lane / LPR;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = (int)blockDim.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = grid.waves;
   int n, hk, grp, split;
   grid.place((int)blockIdx.x, p, &n, &hk, &grp, &split);
   const int h0 = hk * grid.share + grp * G, nh = grid.share - grp * G < G ? grid.share - grp * G : G;
-  const KeyRange all = key_range(p, n), r = split_range(p, all, split);
-  if (p.splits > 1 && split >= used_splits(p, all)) return;
+  const KeyRange all = key_range(p, n);
+  KeyRange r = split_range(p, all, split);
 
   float q[G][VPL], acc[G][VPL], mass[G];
   Query<KD, VPL, LPR, G> qraw;
@@ -364,8 +364,9 @@ __global__ void __launch_bounds__(G == 1 ? 1024 : 512) paged_decode_rows(PagedDe
     }
     if (lane == 0) o[D] = mass[g];
   }
+  if (p.splits > 1 && split >= used_splits(p, all)) return;  // no keys, nobody waits for it
   __syncthreads();
-  for (int i = tid; i < nh * D; i += (int)blockDim.x) {
+  for (int i = tid; i < nh * D; i += 64 * waves) {
     const int g = fdiv(i, grid.dim), d = i - g * D;
     float o = 0.f, m = 0.f;
     for (int w = 0; w < waves; ++w) {
@@ -386,7 +387,7 @@ template <int KD, int VD, int VPL, int LPR, int G, bool ALIGNED>
 void launch_rows_as(const PagedDecodeParams& p, int waves, hipStream_t st) {
   constexpr bool kOne = ALIGNED && G == 1;
   constexpr int U = kOne ? 2 : 1;
-  const DecodeGrid grid(p, G);
+  const DecodeGrid grid(p, G, waves);
   const unsigned n = grid.size(p), threads = 64 * waves, lds = waves * G * (p.D + 1) * sizeof(float);
   if constexpr (kOne) {
     if (p.D == LPR * VPL && grid.alike) {  // what the other form checks costs 5% and more of an e4m3 stream
