@@ -11,9 +11,9 @@
 // Otherwise each lane looks its row's page up.
 //
 // Bound by HBM where the caches are large (bf16 D64, N128 H16 to 4096 ragged
-// tokens, 1.34 GB: 210 us, 6.4 TB/s; e4m3, 0.67 GB: 119 us, 5.7 TB/s), by
-// latency where they are small (N1 H12, 200 keys: 4.3 us, of which an empty
-// sequence takes 3.5).  Loads under way are what counts: a batch of two steps
+// tokens, 1.34 GB: 209 us, 6.4 TB/s; e4m3, 0.68 GB: 118 us, 5.8 TB/s), by
+// latency where they are small (N1 H12, 200 keys: 4.2 us, of which an empty
+// sequence takes 3.3).  Loads under way are what counts: a batch of two steps
 // ahead of the one being added up (four: no faster); eight codes of e4m3 to a
 // lane instead of sixteen halve them and cost 30%.
 #pragma once
