@@ -127,6 +127,7 @@ struct VecGeometry {
   FastDiv heads, tiles, page;
   int ntile;  // groups of R tokens of a sequence
   int units;  // N * ntile * Hk: R tokens of one head
+  bool runs;  // order of the workgroups
 };
 
 template <int CTRL>
@@ -371,10 +372,15 @@ struct Side {
 // Consecutive units are heads of one token, so a wave's rows lie together in
 // the dense tensors, and a thread's tokens lie together in a page.  (Tokens of
 // one head side by side, K and V apart: prompts 73.5 us for 52, read 123 for 62.)
+// Neighbouring workgroups, whose rows share lines of a page, run on one XCD
+// (16 x 256 tokens read 7.3 -> 6.9 us, append of 8 x 4096 tokens to e4m3 52.6 -> 51.7).
 template <bool APPEND, int LPR, int R, bool KF32, bool VF32>
 __global__ void __launch_bounds__(kThreads) paged_rows_vec(PagedRowsParams p, VecGeometry g) {
   const int lane = threadIdx.x % LPR;
-  const int u = blockIdx.x * (kThreads / LPR) + threadIdx.x / LPR;
+  // neighbours on one XCD: all of its share, or runs of eight for many prompts of different lengths
+  const int id = (int)blockIdx.x, in64 = id % 64;
+  const int b = g.runs ? id - in64 + in64 % 8 * 8 + in64 / 8 : xcd_swizzle(id, (int)gridDim.x);
+  const int u = b * (kThreads / LPR) + threadIdx.x / LPR;
   if (u >= g.units) return;
   Places<R> w;
   const int y = fdiv(u, g.heads);
@@ -423,7 +429,10 @@ bool launch_vec(const PagedRowsParams& p, hipStream_t st) {
   auto go = [&](auto lanes) {
     constexpr int LPR = decltype(lanes)::value;
     const int per = kThreads / LPR;
-    paged_rows_vec<APPEND, LPR, R, KF32, VF32><<<(unsigned)((g.units + per - 1) / per), kThreads, 0, st>>>(p, g);
+    unsigned n = (unsigned)((g.units + per - 1) / per);
+    g.runs = APPEND && n >= 2048;
+    n = g.runs ? (n + 63) / 64 * 64 : (n + 7) / 8 * 8;
+    paged_rows_vec<APPEND, LPR, R, KF32, VF32><<<n, kThreads, 0, st>>>(p, g);
     return true;
   };
   if (p.D <= 32) return go(std::integral_constant<int, 4>{});
