@@ -77,6 +77,7 @@ struct DecodeGrid {
   FastDiv page, dim, splits, heads, group_div;
   int share, groups;  // query heads of a key head, and their groups
   int waves;          // of a workgroup
+  int in_runs;        // workgroups taken in runs of eight on one XCD
   // Element strides of pages and rows: a step's place is a few scalar
   // instructions, which a short step waits for as it does for its vector ones.
   uint32_t k0, k2, v0, v2, ke0, ke2, ve0, ve2;
@@ -99,6 +100,9 @@ struct DecodeGrid {
     group_div = fast_div(groups);
     k0 = (uint32_t)p.c.k.s0, k2 = (uint32_t)p.c.k.s2, v0 = (uint32_t)p.c.v.s0, v2 = (uint32_t)p.c.v.s2;
     ke0 = (uint32_t)p.c.ke0, ke2 = (uint32_t)p.c.ke2, ve0 = (uint32_t)p.c.ve0, ve2 = (uint32_t)p.c.ve2;
+    // Key heads side by side share lines of exponent bytes (16 a head at S = 16): one XCD's L2 fetches them once
+    // (e4m3, N128 H16: W256 17.5 -> 16.2 us, 2000 ragged tokens 62.4 -> 60.5; other pages: the same either way).
+    in_runs = p.c.ke ? (int)(size(p) / 64 * 64) : 0;
     alike = k0 == v0 && k2 == v2 && ke0 == ve0 && ke2 == ve2;
   }
   // Elements from the first page's first row to this one's, of a head.
@@ -121,6 +125,7 @@ struct DecodeGrid {
   }
   unsigned size(const PagedDecodeParams& p) const { return (unsigned)((int64_t)p.N * p.Hk * groups * p.splits); }
   __device__ __forceinline__ void place(int b, const PagedDecodeParams& p, int* n, int* hk, int* grp, int* split) const {
+    if (b < in_runs) b = b - b % 64 + b % 8 * 8 + b % 64 / 8;
     int x = fdiv(b, splits);
     *split = b - x * p.splits;
     int y = fdiv(x, group_div);

@@ -11,7 +11,7 @@
 // Otherwise each lane looks its row's page up.
 //
 // Bound by HBM where the caches are large (bf16 D64, N128 H16 to 4096 ragged
-// tokens, 1.34 GB: 209 us, 6.4 TB/s; e4m3, 0.68 GB: 118 us, 5.8 TB/s), by
+// tokens, 1.34 GB: 209 us, 6.4 TB/s; e4m3, 0.68 GB: 116 us, 5.9 TB/s), by
 // latency where they are small (N1 H12, 200 keys: 4.2 us, of which an empty
 // sequence takes 3.3).  Loads under way are what counts: a batch of two steps
 // ahead of the one being added up (four: no faster); eight codes of e4m3 to a
