@@ -178,7 +178,7 @@ def paged_decode(q: Tensor, kv: PagedKV, table: Tensor, lengths: Tensor, scale: 
     of the lengths known on the host, by which the launch is shaped (default:
     what the table can hold); it does not cut a longer sequence.  Sequences
     start in their order: where lengths differ much, longest first is faster
-    (N64 H12, 500 to 2048 e4m3 tokens: 26 us against 29).  Returns out
+    (N64 H12, up to 3000 e4m3 tokens: 34 us against 39).  Returns out
     [N, H, D] in q.dtype, zeros for a sequence with no key."""
     flags = _DECODE_NORMS.get(normalize)
     W = 0 if window is None else int(window)
