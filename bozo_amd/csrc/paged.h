@@ -32,10 +32,9 @@ struct KeyRange {
   int lo, hi;
 };
 
-// Keys of sequence n; the length is held to what the table can name.
-__device__ __forceinline__ KeyRange key_range(const PagedDecodeParams& p, int n) {
+// Keys of a sequence; its length is held to what the table can name.
+__device__ __forceinline__ KeyRange key_range(const PagedDecodeParams& p, int len) {
   const int cap = (int)(p.c.table_len > 0x7fffffff / p.c.S ? 0x7fffffff : p.c.table_len * p.c.S);
-  int len = p.lengths[n];
   len = len < 0 ? 0 : len > cap ? cap : len;
   const int hi = (p.flags & TENSION_DECODE_SELF) ? len : len - 1;
   const int lo = p.W > 0 && len - 1 > p.W ? len - 1 - p.W : 0;
@@ -72,12 +71,59 @@ __device__ __forceinline__ float* split_mass(const PagedDecodeParams& p, int nh,
 // Scale of an exponent byte.
 __device__ __forceinline__ float pow2_of_byte(int b) { return __builtin_bit_cast(float, (unsigned)b << 23); }
 
+// The k-th longest of N <= 256 sequences, by four bits of their lengths and
+// then by index: a wave counts how many share each longer prefix.
+__device__ __forceinline__ int nth_longest(const int32_t* lengths, int N, int shift, int k, int* len) {
+  constexpr int kMost = 4;
+  const int lane = threadIdx.x & 63;
+  int own[kMost], v[kMost];
+#pragma unroll
+  for (int j = 0; j < kMost; ++j) {
+    const int i = 64 * j + lane;
+    own[j] = lengths[i < N ? i : 0];
+  }
+#pragma unroll
+  for (int j = 0; j < kMost; ++j) {
+    const int x = own[j] >> shift;
+    v[j] = 64 * j + lane < N ? (x < 0 ? 0 : x > 15 ? 15 : x) : -1;
+  }
+  int prefix = 0;
+#pragma unroll
+  for (int bit = 3; bit >= 0; --bit) {
+    const int want = 2 * prefix + 1;
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < kMost; ++j) n += __popcll(__ballot((v[j] >> bit) == want));
+    const bool in = k < n;
+    k -= in ? 0 : n;
+    prefix = in ? want : 2 * prefix;
+  }
+  int found = 0, length = 0;
+#pragma unroll
+  for (int j = 0; j < kMost; ++j) {
+    const uint64_t same = __ballot(v[j] == prefix);
+    const int n = __popcll(same);
+    const int before = __builtin_amdgcn_mbcnt_hi((unsigned)(same >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)same, 0));
+    const uint64_t hit = __ballot(v[j] == prefix && before == k);
+    const int at = (int)__builtin_ctzll(hit | (1ull << 63));
+    const int l = __builtin_amdgcn_readlane(own[j], at);
+    const bool here = k >= 0 && k < n;
+    found = here ? 64 * j + at : found;
+    length = here ? l : length;
+    k -= n;
+  }
+  *len = __builtin_amdgcn_readfirstlane(length);
+  return __builtin_amdgcn_readfirstlane(found);
+}
+
 // Workgroups of a decode call: (sequence, key head, group of query heads, split).
 struct DecodeGrid {
-  FastDiv page, dim, splits, heads, group_div;
+  FastDiv page, dim, splits, heads, group_div, fill;
   int share, groups;  // query heads of a key head, and their groups
   int waves;          // of a workgroup
   int in_runs;        // workgroups taken in runs of eight on one XCD
+  int turn;           // sequences that give each CU one workgroup; 0: sequences in their order
+  int shift;
   // Element strides of pages and rows: a step's place is a few scalar
   // instructions, which a short step waits for as it does for its vector ones.
   uint32_t k0, k2, v0, v2, ke0, ke2, ve0, ve2;
@@ -102,6 +148,16 @@ struct DecodeGrid {
     ke0 = (uint32_t)p.c.ke0, ke2 = (uint32_t)p.c.ke2, ve0 = (uint32_t)p.c.ve0, ve2 = (uint32_t)p.c.ve2;
     // Key heads side by side share lines of exponent bytes (16 a head at S = 16): one XCD's L2 fetches them once
     // (e4m3, N128 H16: W256 17.5 -> 16.2 us, 2000 ragged tokens 62.4 -> 60.5; other pages: the same either way).
+    // Where CUs take several workgroups of whole sequences the longest go first, and the next fill of the CUs in
+    // reverse, so that each gets its share.  Finding them stands before every load, so only for calls that may read 100
+    // MB (us, in the sequences' order / so: ragged N128 H16 L2000 e4m3 60.4 / 55.9, N32 L4096 float32 114 / 106, N128
+    // L4096 bf16 209.6 / 204; all of one length, N64 H12 L1000 bf16, 32.3 / 32.8).
+    const int64_t cus = device_cus(), per = (int64_t)p.Hk * groups * p.splits;
+    const float bytes = (float)p.N * (float)p.Hk * (float)p.most * (float)(p.D * (p.c.ke ? 2 : 4));
+    turn = p.W == 0 && p.N > 1 && p.N <= 256 && p.N * per > cus && bytes > 100e6f ? (int)((cus + per - 1) / per) : 0;
+    fill = fast_div(turn > 0 ? turn : 1);
+    shift = 0;
+    while ((p.most >> shift) > 15) ++shift;
     in_runs = p.c.ke ? (int)(size(p) / 64 * 64) : 0;
     alike = k0 == v0 && k2 == v2 && ke0 == ve0 && ke2 == ve2;
   }
@@ -124,14 +180,21 @@ struct DecodeGrid {
     return w;
   }
   unsigned size(const PagedDecodeParams& p) const { return (unsigned)((int64_t)p.N * p.Hk * groups * p.splits); }
-  __device__ __forceinline__ void place(int b, const PagedDecodeParams& p, int* n, int* hk, int* grp, int* split) const {
+  __device__ __forceinline__ void place(int b, const PagedDecodeParams& p, int* n, int* len, int* hk, int* grp, int* split) const {
     if (b < in_runs) b = b - b % 64 + b % 8 * 8 + b % 64 / 8;
     int x = fdiv(b, splits);
     *split = b - x * p.splits;
     int y = fdiv(x, group_div);
     *grp = x - y * groups;
-    *n = fdiv(y, heads);
-    *hk = y - *n * p.Hk;
+    const int z = fdiv(y, heads);
+    *hk = y - z * p.Hk;
+    if (turn) {
+      const int f = fdiv(z, fill), a = f * turn, e = a + turn < p.N ? a + turn : p.N;
+      *n = nth_longest(p.lengths, p.N, shift, f & 1 ? e - 1 - (z - a) : z, len);
+    } else {
+      *n = z;
+      *len = p.lengths[z];
+    }
   }
 };
 

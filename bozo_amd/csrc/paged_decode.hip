@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(64 * kWaves) paged_decode_any(PagedDecodeParam
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, ch = lane & 15;
   const int i = blockIdx.x % p.splits, nh = blockIdx.x / p.splits;
   const int n = nh / p.H, h = nh % p.H, hk = h / (p.H / p.Hk);
-  const KeyRange all = key_range(p, n), r = split_range(p, all, i);
+  const KeyRange all = key_range(p, p.lengths[n]), r = split_range(p, all, i);
   if (p.splits > 1 && i >= used_splits(p, all)) return;
   unsigned kw[VPL], vw[VPL];
   float q[VPL], acc[VPL], x[VPL], mass = 0.f;
@@ -110,7 +110,7 @@ template <int DP, int GROUPS>
 __global__ void __launch_bounds__(DP* GROUPS) paged_decode_join(PagedDecodeParams p) {
   __shared__ float red[GROUPS][DP], mred[DP * GROUPS / 64];
   const int nh = blockIdx.x, n = nh / p.H, h = nh % p.H, tid = threadIdx.x, d = tid % DP, g = tid / DP;
-  const KeyRange all = key_range(p, n);
+  const KeyRange all = key_range(p, p.lengths[n]);
   const int used = used_splits(p, all);
   float m = 0.f, acc = 0.f;
   const float* mass = split_mass(p, nh, 0);

@@ -72,10 +72,10 @@ __global__ void __launch_bounds__(64 * kWaves, F8 || D == 64 ? 3 : 2) paged_deco
   __shared__ float red[kWaves][16][D + 1];
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int n, hk, grp, split;
-  grid.place((int)blockIdx.x, p, &n, &hk, &grp, &split);
+  int n, len, hk, grp, split;
+  grid.place((int)blockIdx.x, p, &n, &len, &hk, &grp, &split);
   const int h0 = hk * grid.share + grp * 16, nh = grid.share - grp * 16 < 16 ? grid.share - grp * 16 : 16;
-  const KeyRange all = key_range(p, n), r = split_range(p, all, split);
+  const KeyRange all = key_range(p, len), r = split_range(p, all, split);
   if (p.splits > 1 && split >= used_splits(p, all)) return;
 
   const char* kbase = (const char*)p.c.k.p + (int64_t)hk * p.c.k.s1 * kElt;

@@ -11,7 +11,7 @@
 // Otherwise each lane looks its row's page up.
 //
 // Bound by HBM where the caches are large (bf16 D64, N128 H16 to 4096 ragged
-// tokens, 1.34 GB: 209 us, 6.4 TB/s; e4m3, 0.68 GB: 116 us, 5.9 TB/s), by
+// tokens, 1.34 GB: 204 us, 6.6 TB/s; e4m3, 0.68 GB: 109 us, 6.3 TB/s), by
 // latency where they are small (N1 H12, 200 keys: 4.2 us, of which an empty
 // sequence takes 3.3).  Loads under way are what counts: a batch of two steps
 // ahead of the one being added up (four: no faster); eight codes of e4m3 to a
@@ -222,10 +222,10 @@ __global__ void __launch_bounds__(G == 1 ? 1024 : 512) paged_decode_rows(PagedDe
   extern __shared__ float red[];  // [waves][G][D + 1]
   const int tid = threadIdx.x, lane = tid & 63, ch = lane % LPR, lr = lane / LPR;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = grid.waves;
-  int n, hk, grp, split;
-  grid.place((int)blockIdx.x, p, &n, &hk, &grp, &split);
+  int n, len, hk, grp, split;
+  grid.place((int)blockIdx.x, p, &n, &len, &hk, &grp, &split);
   const int h0 = hk * grid.share + grp * G, nh = grid.share - grp * G < G ? grid.share - grp * G : G;
-  const KeyRange all = key_range(p, n);
+  const KeyRange all = key_range(p, len);
   KeyRange r = split_range(p, all, split);
 
   float q[G][VPL], acc[G][VPL], mass[G];

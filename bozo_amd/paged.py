@@ -176,9 +176,7 @@ def paged_decode(q: Tensor, kv: PagedKV, table: Tensor, lengths: Tensor, scale: 
     range) or None / "raw", as in ``decode_step``.  H may be a multiple of the
     pages' heads: query head h reads key head h // (H / Hk).  max_len: a bound
     of the lengths known on the host, by which the launch is shaped (default:
-    what the table can hold); it does not cut a longer sequence.  Sequences
-    start in their order: where lengths differ much, longest first is faster
-    (N64 H12, up to 3000 e4m3 tokens: 34 us against 39).  Returns out
+    what the table can hold); it does not cut a longer sequence.  Returns out
     [N, H, D] in q.dtype, zeros for a sequence with no key."""
     flags = _DECODE_NORMS.get(normalize)
     W = 0 if window is None else int(window)

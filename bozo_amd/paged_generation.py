@@ -227,15 +227,8 @@ class TensionPagedCache:
     @torch.no_grad()
     def step(self, seqs: Sequence[int], next_ids: Tensor) -> Tensor:
         """Advance these sequences by one token each (ids [N]), every one at
-        its own position; returns their logits [N, vocab].  They are taken
-        longest first, which shares them out among the CUs."""
+        its own position; returns their logits [N, vocab]."""
         self._live(seqs)
-        order = sorted(range(len(seqs)), key=lambda i: -self.length[seqs[i]])
-        if order != list(range(len(seqs))):
-            back = torch.empty(len(seqs), dtype=torch.long)
-            back[order] = torch.arange(len(seqs))
-            logits = self.step([seqs[i] for i in order], next_ids[torch.tensor(order, device=next_ids.device)])
-            return logits[back.to(logits.device)]
         self._ready(seqs, [1] * len(seqs))
         model, dev = self.model, self.lengths.device
         N = len(seqs)

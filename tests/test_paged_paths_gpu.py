@@ -105,6 +105,24 @@ def test_rows_head_dims_in_eights(src, pages, D):
         check_decode(q * 0.1, fill(kv, 2), table, lengths, math.sqrt(D))
 
 
+@pytest.mark.parametrize("q,pages,share", [("bf16", "bf16", 1), ("bf16", "e4m3", 1), ("f32", "f32", 1), ("bf16", "e4m3", 4),
+                                           ("f32", "f32", 2)])
+@pytest.mark.parametrize("N,Hk", [(65, 4), (64, 5), (256, 2), (200, 2), (257, 2), (3, 100), (2, 300)])
+def test_sequences_taken_by_length(q, pages, share, N, Hk):
+    """Large calls take the longest sequences first: every one once, whatever
+    its length (empty, below zero, alike, past the bound that shapes the call)."""
+    g = np.random.default_rng(N)
+    lengths = g.choice([0, 1, 2, 3, 17, 40, 90, 130, 131], N)
+    lengths[g.integers(N)] = 400
+    table, P = make_table(lengths.tolist(), 16, seed=N, width=60000)
+    kv = fill(PagedKV.empty(P, 16, Hk, 64, DT[pages]), N)
+    x = query(N, Hk * share, 64, q)
+    check_decode(x, kv, table, lengths, 8.0, max_len=20000)
+    check_decode(x, kv, table, lengths, 8.0, max_len=300000, norm="count")
+    lengths[g.integers(N)] = -5
+    check_decode(x, kv, table, lengths, 8.0)
+
+
 @pytest.mark.parametrize("pages,q,share", [("bf16", "bf16", 1), ("bf16", "bf16", 4), ("e4m3", "bf16", 1), ("e4m3", "f16", 2),
                                            ("f32", "f32", 1), ("f16", "f16", 2)])
 def test_values_in_another_order(pages, q, share):
