@@ -1,8 +1,8 @@
 // Paged K/V cache: tokens written into pages (quantised to e4m3 on the way or
 // as they are) and read back dense.  Both are streams: a row of D values is
-// read once and written once, so HBM bounds them (bf16 prompts, 262 MB: 52 us,
-// 5.0 TB/s, what a large copy reaches; e4m3 read back, 303 MB: 62 to 67 us), and
-// below some 20 MB the chain of start, table, rows (about 4 us).
+// read once and written once, so HBM bounds them (bf16 prompts, 262 MB: 50 us,
+// 5.3 TB/s, what a large copy reaches; e4m3 read back, 303 MB: 65 us), and below
+// some 20 MB the chain of start, table, rows (about 4 us).
 //
 // Quantised rows: with E the biased exponent of a row's largest finite
 // magnitude a and M its mantissa bits, 448 = 1.75 * 2^8 gives the smallest e
@@ -178,6 +178,14 @@ __device__ __forceinline__ u32x4 rounded_as(const float* x) {
   return __builtin_bit_cast(u32x4, h);
 }
 
+// A store past the L2s, whose lines a kernel has to write back at its end
+// anyway: 16 x 256 tokens read 7.1 -> 5.6 us, 19.6 -> 18.9 with the kernel that
+// reads the result; bf16 prompts 52.5 -> 49.6, 105.1 -> 103.3 with their read.
+template <typename V>
+__device__ __forceinline__ void stream(void* p, V v) {
+  __builtin_nontemporal_store(v, (V*)p);
+}
+
 // Eight values of a row of float32 (WIDE) or 16-bit type, as they are loaded.
 template <bool WIDE>
 struct Eight {
@@ -196,13 +204,13 @@ struct Eight {
   __device__ __forceinline__ void store(const Buf& b, int64_t off, Quads q) const {
     void* p = const_cast<void*>(b.p);
     if constexpr (WIDE) {
-      *(u32x4*)((float*)p + off + q.a) = a[0];
-      *(u32x4*)((float*)p + off + q.b) = a[1];
+      stream((float*)p + off + q.a, a[0]);
+      stream((float*)p + off + q.b, a[1]);
     } else if (q.b == q.a + 4) {
-      *(u32x4*)((f16*)p + off + q.a) = a[0];
+      stream((f16*)p + off + q.a, a[0]);
     } else {
-      *(u32x2*)((f16*)p + off + q.a) = u32x2{a[0][0], a[0][1]};
-      *(u32x2*)((f16*)p + off + q.b) = u32x2{a[0][2], a[0][3]};
+      stream((f16*)p + off + q.a, u32x2{a[0][0], a[0][1]});
+      stream((f16*)p + off + q.b, u32x2{a[0][2], a[0][3]});
     }
   }
   __device__ __forceinline__ void zero() {
@@ -373,7 +381,7 @@ struct Side {
 // the dense tensors, and a thread's tokens lie together in a page.  (Tokens of
 // one head side by side, K and V apart: prompts 73.5 us for 52, read 123 for 62.)
 // Neighbouring workgroups, whose rows share lines of a page, run on one XCD
-// (16 x 256 tokens read 7.3 -> 6.9 us, append of 8 x 4096 tokens to e4m3 52.6 -> 51.7).
+// (16 x 256 tokens read 7.3 -> 6.9 us then, append of 8 x 4096 tokens to e4m3 52.6 -> 51.7).
 template <bool APPEND, int LPR, int R, bool KF32, bool VF32>
 __global__ void __launch_bounds__(kThreads) paged_rows_vec(PagedRowsParams p, VecGeometry g) {
   const int lane = threadIdx.x % LPR;
