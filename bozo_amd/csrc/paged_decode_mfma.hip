@@ -12,7 +12,7 @@
 //
 // Roundings: K, q and V enter as they are (an e4m3 code is a bf16 and an f16
 // number; its row's scale is applied to the score, or to tau).  tau enters as
-// two bf16 terms, off by 2^-16 of itself at most; sums are float32.
+// three bf16 terms that make up its float32 value; sums are float32.
 //
 // Bound by HBM: 32 keys of 128 e4m3 values (8.3 KB) take a wave about 900 cycles
 // of vector instructions, a quarter of what the card's rate leaves it; the time
@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(64 * kWaves, F8 || D == 64 ? 3 : 2) paged_deco
           every = every && ok[t][i];
         }
       const bool whole = __all(every);
-      // tau as two bf16 terms, in A's order
+      // tau, in A's order
       float tau[2][4];
 #pragma unroll
       for (int t = 0; t < 2; ++t)
@@ -199,21 +199,23 @@ __global__ void __launch_bounds__(64 * kWaves, F8 || D == 64 ? 3 : 2) paged_deco
           if constexpr (F8) x = ok[t][i] ? x * pow2_of_byte((ve[t] >> (8 * i)) & 0xff) : 0.f;
           tau[t][i] = x;
         }
-      u32x4 th, tl;
+      // Three bf16 terms make up tau exactly: each of the first two is less than what is left and all are positive, so
+      // an infinite value row stays infinite; the last has 8 significant bits at most.
+      u32x4 term[3];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        // the first term is less than tau and the second positive: an infinite value row stays infinite
-        unsigned hi2 = 0;
-        bf16x2 lo2;
+        unsigned w[3][2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const float x = tau[j / 2][2 * (j % 2) + e];
-          const unsigned w = x == 0.f ? 0u : (__builtin_bit_cast(unsigned, x) - 1) & 0xffff0000u;
-          hi2 |= e ? w : w >> 16;
-          lo2[e] = (bf16)(x - __builtin_bit_cast(float, w));
+          const unsigned some = x == 0.f ? 0u : 0xffff0000u;
+          w[0][e] = (__builtin_bit_cast(unsigned, x) - 1) & some;
+          const float left = x - __builtin_bit_cast(float, w[0][e]);
+          w[1][e] = (__builtin_bit_cast(unsigned, left) - 1) & some;
+          w[2][e] = __builtin_bit_cast(unsigned, left - __builtin_bit_cast(float, w[1][e]));
         }
-        th[j] = hi2;
-        tl[j] = __builtin_bit_cast(unsigned, lo2);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) term[i][j] = halves<true>(w[i][0], w[i][1]);
       }
       if (!whole) {
 #pragma unroll
@@ -248,8 +250,8 @@ __global__ void __launch_bounds__(64 * kWaves, F8 || D == 64 ? 3 : 2) paged_deco
       }
 #pragma unroll
       for (int j = 0; j < VN; ++j) {
-        acc[j] = product<false>(th, bv[j], acc[j]);
-        acc[j] = product<false>(tl, bv[j], acc[j]);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) acc[j] = product<false>(term[i], bv[j], acc[j]);
       }
     }
   }

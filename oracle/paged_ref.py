@@ -87,7 +87,8 @@ def decode_bound(out, keys, mag, dots, D: int, eps: float) -> np.ndarray:
 
     * a score of D float32 products and the logistic function: (D + 8) 2^-24
       of sum |q k| / scale, plus 8 ulp, relative in tau;
-    * 16-bit results carry tau as two 16-bit terms: 2^-16 relative;
+    * tau as the sums take it: 2^-23 relative; 2^-16 for 16-bit results, room
+      that no kernel needs (tests/test_paged_weights_gpu.py has the tight bound);
     * sums over the keys and the splits: (keys + 16) 2^-24 relative;
     numerator and mass alike (twice), then half a step of the output type."""
     u = 2.0 ** -24
