@@ -136,6 +136,8 @@ class TensionPagedCache:
 
     def _live(self, seqs: Sequence[int]) -> None:
         for s in seqs:
+            if not 0 <= s < len(self.length):
+                raise ValueError(f"no sequence {s}: they are numbered 0 to {len(self.length) - 1}")
             if self.length[s] == 0:
                 raise ValueError(f"sequence {s} is not in use")
 
