@@ -17,6 +17,7 @@ the rounding of the pages' type.
 """
 from __future__ import annotations
 
+from contextlib import contextmanager
 from typing import Optional, Sequence
 
 import torch
@@ -49,25 +50,26 @@ class PageTable:
         a, b = self._span(length, more)
         return int((self.rows[seq, a:b] < 0).sum())
 
-    def grow(self, seq: int, length: int, more: int) -> None:
+    def grow(self, seq: int, length: int, more: int) -> list:
         """Pages for tokens length .. length + more - 1 (those in the window
-        of what follows them)."""
+        of what follows them).  Returns the entries it filled."""
         a, b = self._span(length, more)
-        for i in range(a, b):
-            if self.rows[seq, i] < 0:
-                self.rows[seq, i] = self.free.pop()
-                self.changed = True
+        new = [i for i in range(a, b) if self.rows[seq, i] < 0]
+        for i in new:
+            self.rows[seq, i] = self.free.pop()
+            self.changed = True
+        return new
 
     def drop(self, seq: int, length: int) -> None:
         """Hand on the pages that no token from position ``length`` reads."""
         if self.window:
-            self._give(seq, 0, max(0, length - self.window) // self.S)
+            self.give(seq, range(max(0, length - self.window) // self.S))
 
     def release(self, seq: int) -> None:
-        self._give(seq, 0, self.rows.shape[1])
+        self.give(seq, range(self.rows.shape[1]))
 
-    def _give(self, seq: int, a: int, b: int) -> None:
-        for i in range(a, b):
+    def give(self, seq: int, entries) -> None:
+        for i in entries:
             if self.rows[seq, i] >= 0:
                 self.free.append(int(self.rows[seq, i]))
                 self.rows[seq, i] = -1
@@ -102,8 +104,10 @@ class TensionPagedCache:
 
     # ---------------------------------------------------------------- bookkeeping
 
-    def _ready(self, seqs: Sequence[int], more: Sequence[int]) -> None:
-        """Room for the call's tokens, or an error before anything changes."""
+    @contextmanager
+    def _room(self, seqs: Sequence[int], more: Sequence[int]):
+        """Room for the call's tokens, or an error before anything changes.
+        The pages taken for them go back if what follows fails."""
         if self.model.training:
             raise RuntimeError("generation needs model.eval() (dropout off)")
         if len(set(seqs)) != len(seqs):
@@ -115,9 +119,13 @@ class TensionPagedCache:
         for t in self.tables.values():
             if sum(t.missing(s, self.length[s], m) for s, m in zip(seqs, more)) > len(t.free):
                 raise RuntimeError(f"out of pages ({t.pages} in the pool): release a sequence, or wait for one to end")
-        for t in self.tables.values():
-            for s, m in zip(seqs, more):
-                t.grow(s, self.length[s], m)
+        taken = [(t, s, t.grow(s, self.length[s], m)) for t in self.tables.values() for s, m in zip(seqs, more)]
+        try:
+            yield
+        except BaseException:
+            for t, s, entries in reversed(taken):
+                t.give(s, reversed(entries))
+            raise
 
     def _rows(self, idx: Tensor) -> dict:
         """The tables' rows of these sequences, on the device."""
@@ -167,28 +175,29 @@ class TensionPagedCache:
         if len(seqs) < len(prompts):
             raise RuntimeError(f"{len(prompts)} prompts for {len(seqs)} free sequences")
         counts = [int(p.numel()) for p in prompts]
-        self._ready(seqs, counts)
-        dev = self.lengths.device
-        ids = torch.zeros(len(prompts), max(counts), dtype=torch.long)
-        for row, p in zip(ids, prompts):
-            row[:p.numel()] = p
-        idx = torch.tensor(seqs, device=dev)
-        n = torch.tensor(counts, dtype=torch.int32, device=dev)
-        start, rows = torch.zeros_like(n), self._rows(idx)
+        with self._room(seqs, counts):
+            dev = self.lengths.device
+            ids = torch.zeros(len(prompts), max(counts), dtype=torch.long)
+            for row, p in zip(ids, prompts):
+                row[:p.numel()] = p
+            idx = torch.tensor(seqs, device=dev)
+            n = torch.tensor(counts, dtype=torch.int32, device=dev)
+            start, rows = torch.zeros_like(n), self._rows(idx)
 
-        def store(i, k, v):
-            paged_append(self._pages(i, k, v), k, v, rows[self.model.blocks[i].global_layer], start, n)
+            def store(i, k, v):
+                paged_append(self._pages(i, k, v), k, v, rows[self.model.blocks[i].global_layer], start, n)
 
-        layers = [b.tension for b in self.model.blocks]
-        for i, layer in enumerate(layers):
-            layer.kv_sink = (lambda k, v, i=i: store(i, k, v))
-        try:
-            logits = self.model(ids.to(dev))
-        finally:
-            for layer in layers:
-                layer.kv_sink = None
-        self._advance(seqs, counts, idx, n)
-        return seqs, logits[torch.arange(len(seqs), device=dev), n.long() - 1]
+            layers = [b.tension for b in self.model.blocks]
+            for i, layer in enumerate(layers):
+                layer.kv_sink = (lambda k, v, i=i: store(i, k, v))
+            try:
+                logits = self.model(ids.to(dev))
+            finally:
+                for layer in layers:
+                    layer.kv_sink = None
+            last = logits[torch.arange(len(seqs), device=dev), n.long() - 1]
+            self._advance(seqs, counts, idx, n)
+            return seqs, last
 
     @torch.no_grad()
     def extend(self, seq: int, ids: Tensor) -> Tensor:
@@ -197,71 +206,74 @@ class TensionPagedCache:
         the keys and values before them back from its pages."""
         self._live([seq])
         T, t0 = int(ids.numel()), self.length[seq]
-        self._ready([seq], [T])
-        model, dev = self.model, self.lengths.device
-        idx = torch.tensor([seq], device=dev)
-        rows, start = self._rows(idx), self.lengths.index_select(0, idx)
-        at = torch.arange(t0, t0 + T, device=dev)
-        x = model.embedding(ids.to(dev).view(1, T))
-        if model.pos_embedding is not None:
-            x = x + model.pos_embedding(at)[None]
-        fpos = _osc_positions(model, at)
-        for i, blk in enumerate(model.blocks):
-            layer, h = blk.tension, blk.pre_norm(x)
-            q, k, v = layer._qkv(h, t0)
-            if blk.global_layer:
-                q, k, v = autocast_inputs(q, k, v)
-            table, kv = rows[blk.global_layer], self._pages(i, k, v)
-            before = t0 if blk.global_layer else min(t0, layer.window)
-            kp, vp = paged_read(kv, table, start - before, before, (k.dtype, v.dtype))
-            paged_append(kv, k, v, table, start)
-            q = torch.cat([q.new_zeros(1, before, *q.shape[2:]), q], 1)  # the rows before are not asked for
-            k, v = torch.cat([kp, k], 1), torch.cat([vp, v], 1)
-            if blk.global_layer:
-                out = global_tension(q, k, v, layer.scale)
-            else:
-                out = causal_tension(q, k, v, layer.window, layer.scale, normalize="count" if layer.count_norm else "mass")
-            h = layer.norm(h + layer.wo(out[:, before:].reshape(1, T, -1)))
-            x = _after_tension(blk, h, fpos)
-        self._advance([seq], [T], idx, start + T)
-        return model.lm_head(model.final_norm(x[:, -1]))[0]
+        with self._room([seq], [T]):
+            model, dev = self.model, self.lengths.device
+            idx = torch.tensor([seq], device=dev)
+            rows, start = self._rows(idx), self.lengths.index_select(0, idx)
+            at = torch.arange(t0, t0 + T, device=dev)
+            x = model.embedding(ids.to(dev).view(1, T))
+            if model.pos_embedding is not None:
+                x = x + model.pos_embedding(at)[None]
+            fpos = _osc_positions(model, at)
+            for i, blk in enumerate(model.blocks):
+                layer, h = blk.tension, blk.pre_norm(x)
+                q, k, v = layer._qkv(h, t0)
+                if blk.global_layer:
+                    q, k, v = autocast_inputs(q, k, v)
+                table, kv = rows[blk.global_layer], self._pages(i, k, v)
+                before = t0 if blk.global_layer else min(t0, layer.window)
+                kp, vp = paged_read(kv, table, start - before, before, (k.dtype, v.dtype))
+                paged_append(kv, k, v, table, start)
+                q = torch.cat([q.new_zeros(1, before, *q.shape[2:]), q], 1)  # the rows before are not asked for
+                k, v = torch.cat([kp, k], 1), torch.cat([vp, v], 1)
+                if blk.global_layer:
+                    out = global_tension(q, k, v, layer.scale)
+                else:
+                    out = causal_tension(q, k, v, layer.window, layer.scale,
+                                         normalize="count" if layer.count_norm else "mass")
+                h = layer.norm(h + layer.wo(out[:, before:].reshape(1, T, -1)))
+                x = _after_tension(blk, h, fpos)
+            logits = model.lm_head(model.final_norm(x[:, -1]))[0]
+            self._advance([seq], [T], idx, start + T)
+            return logits
 
     @torch.no_grad()
     def step(self, seqs: Sequence[int], next_ids: Tensor) -> Tensor:
         """Advance these sequences by one token each (ids [N]), every one at
         its own position; returns their logits [N, vocab]."""
         self._live(seqs)
-        self._ready(seqs, [1] * len(seqs))
-        model, dev = self.model, self.lengths.device
-        N = len(seqs)
-        idx = torch.tensor(seqs, device=dev)
-        rows = self._rows(idx)
-        pos = self.lengths.index_select(0, idx)
-        lengths, at = pos + 1, pos.long()
-        most = max(self.length[s] for s in seqs) + 1
-        x = model.embedding(next_ids.to(dev).view(N, 1))
-        if model.pos_embedding is not None:
-            x = x + model.pos_embedding(at)[:, None]
-        fpos = _osc_positions(model, at)
-        fpos = None if fpos is None else fpos[:, None]
-        first = model.blocks[0].tension
-        rot = None
-        if first.rope_enabled:  # one row of the tables a sequence
-            rot = (first.rope.cos.index_select(0, at), first.rope.sin.index_select(0, at))
-        for i, blk in enumerate(model.blocks):
-            layer, h = blk.tension, blk.pre_norm(x)
-            q, k, v = _step_qkv(layer, h, rot)
-            kv, table = self._pages(i, k, v), rows[blk.global_layer]
-            paged_append(kv, k[:, None], v[:, None], table, pos)
-            if blk.global_layer:
-                out = paged_decode(q, kv, table, lengths, layer.scale, max_len=most)
-            else:
-                out = paged_decode(q, kv, table, lengths, layer.scale, window=layer.window, include_self=False,
-                                   normalize="count" if layer.count_norm else "mass", max_len=most)
-            h = layer.norm(h + layer.wo(out.reshape(N, 1, -1)).to(h.dtype))
-            x = _after_tension(blk, h, fpos)
-        self._advance(seqs, [1] * N, idx, lengths)
-        return model.lm_head(model.final_norm(x))[:, 0]
+        with self._room(seqs, [1] * len(seqs)):
+            model, dev = self.model, self.lengths.device
+            N = len(seqs)
+            idx = torch.tensor(seqs, device=dev)
+            rows = self._rows(idx)
+            pos = self.lengths.index_select(0, idx)
+            lengths, at = pos + 1, pos.long()
+            most = max(self.length[s] for s in seqs) + 1
+            x = model.embedding(next_ids.to(dev).view(N, 1))
+            if model.pos_embedding is not None:
+                x = x + model.pos_embedding(at)[:, None]
+            fpos = _osc_positions(model, at)
+            fpos = None if fpos is None else fpos[:, None]
+            first = model.blocks[0].tension
+            rot = None
+            if first.rope_enabled:  # one row of the tables a sequence
+                rot = (first.rope.cos.index_select(0, at), first.rope.sin.index_select(0, at))
+            for i, blk in enumerate(model.blocks):
+                layer, h = blk.tension, blk.pre_norm(x)
+                q, k, v = _step_qkv(layer, h, rot)
+                kv, table = self._pages(i, k, v), rows[blk.global_layer]
+                paged_append(kv, k[:, None], v[:, None], table, pos)
+                if blk.global_layer:
+                    out = paged_decode(q, kv, table, lengths, layer.scale, max_len=most)
+                else:
+                    out = paged_decode(q, kv, table, lengths, layer.scale, window=layer.window, include_self=False,
+                                       normalize="count" if layer.count_norm else "mass", max_len=most)
+                h = layer.norm(h + layer.wo(out.reshape(N, 1, -1)).to(h.dtype))
+                x = _after_tension(blk, h, fpos)
+            logits = model.lm_head(model.final_norm(x))[:, 0]
+            self._advance(seqs, [1] * N, idx, lengths)
+            return logits
 
 
 def _step_qkv(layer, x: Tensor, rot):
