@@ -11,6 +11,7 @@
 //
 // The GIL is released for the whole call, as ctypes does.  Nothing is kept
 // from one call for the next.
+#include <ATen/TracerMode.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -377,11 +378,15 @@ bool counter_ok(const Tensor& t, int64_t N, const Tensor& like) {
 }
 const int32_t* counter_ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr<int32_t>() : nullptr; }
 
-// False when an operand does not fit the others (the caller then says which),
-// likewise below.
+// Whether torch.jit.trace is recording this call (not inside an operator that
+// it recorded already).
+bool recorded() { return at::tracer::impl::is_dispatch_enabled(); }
+
+// False when an operand does not fit the others (the caller then says which)
+// or a trace records, likewise below.
 bool paged_append(const Tensor& k, const Tensor& v, const OptTensor& ke, const OptTensor& ve, const Tensor& kn,
                   const Tensor& vn, const Tensor& table, const Tensor& start, const OptTensor& counts_) {
-  if (kn.dim() != 4 || vn.sizes() != kn.sizes() || !dense_ok(kn.scalar_type()) || !dense_ok(vn.scalar_type()) ||
+  if (recorded() || kn.dim() != 4 || vn.sizes() != kn.sizes() || !dense_ok(kn.scalar_type()) || !dense_ok(vn.scalar_type()) ||
       kn.device() != k.device() || vn.device() != k.device() || k.dim() != 4 || kn.size(2) != k.size(1) ||
       kn.size(3) != k.size(3))
     return false;
@@ -409,7 +414,7 @@ std::optional<std::tuple<Tensor, Tensor>> paged_read(const Tensor& k, const Tens
                                                      const OptTensor& ve, const Tensor& table, const Tensor& start,
                                                      int64_t T, at::ScalarType kdt, at::ScalarType vdt,
                                                      const OptTensor& counts_) {
-  if (T < 0 || !dense_ok(kdt) || !dense_ok(vdt) || start.dim() != 1 || k.dim() != 4 || !k.is_cuda()) return std::nullopt;
+  if (recorded() || T < 0 || !dense_ok(kdt) || !dense_ok(vdt) || start.dim() != 1 || k.dim() != 4 || !k.is_cuda()) return std::nullopt;
   const int64_t N = start.size(0), Hk = k.size(1), D = k.size(3);
   const Tensor counts = opt(counts_);
   if (!counter_ok(start, N, k) || !counter_ok(counts, N, k)) return std::nullopt;
@@ -428,7 +433,7 @@ std::optional<std::tuple<Tensor, Tensor>> paged_read(const Tensor& k, const Tens
 OptTensor paged_decode(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& ke, const OptTensor& ve,
                        const Tensor& table, const Tensor& lengths, double scale, int64_t W, int64_t max_len,
                        int64_t flags) {
-  if (q.dim() != 3 || !q.is_cuda() || !dense_ok(q.scalar_type()) || k.dim() != 4 || q.device() != k.device() ||
+  if (recorded() || q.dim() != 3 || !q.is_cuda() || !dense_ok(q.scalar_type()) || k.dim() != 4 || q.device() != k.device() ||
       q.size(2) != k.size(3) || W < 0 || max_len < 0)
     return std::nullopt;
   const int64_t N = q.size(0), H = q.size(1), D = q.size(2), Hk = k.size(1);

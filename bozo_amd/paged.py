@@ -116,10 +116,20 @@ def paged_append(kv: PagedKV, k_new: Tensor, v_new: Tensor, table: Tensor, start
     table: int32 [N, pages per sequence]; start, counts: int32 [N], all on
     the GPU.  Positions that the table has no page for are left out.  The
     pages that are written must belong to one sequence each."""
-    if not L.host().paged_append(*kv, k_new, v_new, table, start, counts):
-        _on_gpu(*kv, k_new, v_new, table, start, counts)
-        _check_append(kv, k_new, v_new, table, start, counts)
-        raise ValueError("paged_append: operands do not fit")
+    args = (*kv, k_new, v_new, table, start, counts)
+    if L.host().paged_append(*args):
+        return
+    if torch.jit.is_tracing():
+        torch.ops.bozo.paged_append(*args)
+    else:
+        _refuse_append(*args)
+
+
+def _refuse_append(k, v, k_exp, v_exp, k_new, v_new, table, start, counts) -> None:
+    kv = (k, v, k_exp, v_exp)
+    _on_gpu(*kv, k_new, v_new, table, start, counts)
+    _check_append(kv, k_new, v_new, table, start, counts)
+    raise ValueError("paged_append: operands do not fit")
 
 
 def paged_read(kv: PagedKV, table: Tensor, start: Tensor, T: int,
@@ -132,11 +142,19 @@ def paged_read(kv: PagedKV, table: Tensor, start: Tensor, T: int,
     kd, vd = dtype if isinstance(dtype, tuple) else (dtype, dtype)
     kd = kd or (torch.bfloat16 if kv[0].dtype == torch.float8_e4m3fn else kv[0].dtype)
     vd = vd or (torch.bfloat16 if kv[1].dtype == torch.float8_e4m3fn else kv[1].dtype)
-    res = L.host().paged_read(*kv, table, start, int(T), kd, vd, counts)
+    args = (*kv, table, start, int(T), kd, vd, counts)
+    res = L.host().paged_read(*args)
     if res is not None:
         return res
+    if torch.jit.is_tracing():
+        return torch.ops.bozo.paged_read(*args)
+    _refuse_read(*args)
+
+
+def _refuse_read(k, v, k_exp, v_exp, table, start, T: int, kd, vd, counts) -> None:
+    kv = (k, v, k_exp, v_exp)
     _on_gpu(*kv, table, start, counts)
-    if int(T) < 0:
+    if T < 0:
         raise ValueError("T must be >= 0")
     if start.dim() != 1:
         raise ValueError(f"start must be int32 [N], got {list(start.shape)}")
@@ -184,10 +202,48 @@ def paged_decode(q: Tensor, kv: PagedKV, table: Tensor, lengths: Tensor, scale: 
     if window is not None and W < 1:
         raise ValueError("window must be >= 1")
     if flags is not None:
-        out = L.host().paged_decode(q, *kv, table, lengths, float(scale), W, most,
-                                    flags | (L.DECODE_SELF if include_self else 0))
+        args = (q, *kv, table, lengths, float(scale), W, most, flags | (L.DECODE_SELF if include_self else 0))
+        out = L.host().paged_decode(*args)
         if out is not None:
             return out
+        if torch.jit.is_tracing():
+            return torch.ops.bozo.paged_decode(*args)
+    _refuse_decode(q, kv, table, lengths, W, most)
+
+
+def _refuse_decode(q, kv, table, lengths, W, most) -> None:
     _on_gpu(q, *kv, table, lengths)
     _check_decode(q, kv, table, lengths, W, most)
     raise ValueError(f"normalize must be one of {list(_DECODE_NORMS)}")
+
+
+# ----------------------------------------------------------------- torch.library registration
+#
+# torch.jit.trace records what goes through the dispatcher.  The native call
+# path sends nothing there but the outputs' allocation, which a replay would
+# hand out as it is: it refuses while a trace records, and the call goes
+# through these.
+
+@torch.library.custom_op("bozo::paged_append", mutates_args=("k", "v", "k_exp", "v_exp"), device_types="cuda")
+def _op_append(k: Tensor, v: Tensor, k_exp: Optional[Tensor], v_exp: Optional[Tensor], k_new: Tensor, v_new: Tensor,
+               table: Tensor, start: Tensor, counts: Optional[Tensor]) -> None:
+    args = (k, v, k_exp, v_exp, k_new, v_new, table, start, counts)
+    if not L.host().paged_append(*args):
+        _refuse_append(*args)
+
+
+@torch.library.custom_op("bozo::paged_read", mutates_args=(), device_types="cuda")
+def _op_read(k: Tensor, v: Tensor, k_exp: Optional[Tensor], v_exp: Optional[Tensor], table: Tensor, start: Tensor,
+             T: int, k_dtype: torch.dtype, v_dtype: torch.dtype, counts: Optional[Tensor]) -> tuple[Tensor, Tensor]:
+    args = (k, v, k_exp, v_exp, table, start, T, k_dtype, v_dtype, counts)
+    return L.host().paged_read(*args) or _refuse_read(*args)
+
+
+@torch.library.custom_op("bozo::paged_decode", mutates_args=(), device_types="cuda")
+def _op_decode(q: Tensor, k: Tensor, v: Tensor, k_exp: Optional[Tensor], v_exp: Optional[Tensor], table: Tensor,
+               lengths: Tensor, scale: float, W: int, most: int, flags: int) -> Tensor:
+    kv = (k, v, k_exp, v_exp)
+    out = L.host().paged_decode(q, *kv, table, lengths, scale, W, most, flags)
+    if out is None:
+        _refuse_decode(q, kv, table, lengths, W, most)
+    return out
