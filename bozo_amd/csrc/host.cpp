@@ -291,13 +291,17 @@ struct RopeFn : torch::autograd::Function<RopeFn> {
 
 // ------------------------------------------------------------------- decode
 
+// Whether torch.jit.trace is recording this call (not inside an operator that
+// it recorded already).
+bool recorded() { return at::tracer::impl::is_dispatch_enabled(); }
+
 // One step, or nothing when an operand does not fit the others (the caller
-// then says which).
+// then says which) or a trace records.
 OptTensor decode_step(const Tensor& q, const Tensor& kn, const Tensor& vn, const Tensor& kc, const Tensor& vc,
                       const Tensor& pos_in, const OptTensor& pos_out_, double scale, int64_t flags,
                       const OptTensor& tau_) {
   const Tensor pos_out = opt(pos_out_), tau = opt(tau_);
-  if (q.dim() != 3 || kc.dim() != 4 || !q.is_cuda()) return std::nullopt;
+  if (recorded() || q.dim() != 3 || kc.dim() != 4 || !q.is_cuda()) return std::nullopt;
   const int64_t N = q.size(0), H = q.size(1), D = q.size(2), W = kc.size(2);
   auto same = [&](const Tensor& t) { return !t.defined() || t.device() == q.device(); };
   auto counter = [&](const Tensor& t) {
@@ -377,10 +381,6 @@ bool counter_ok(const Tensor& t, int64_t N, const Tensor& like) {
   return !t.defined() || (t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == N && t.device() == like.device());
 }
 const int32_t* counter_ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr<int32_t>() : nullptr; }
-
-// Whether torch.jit.trace is recording this call (not inside an operator that
-// it recorded already).
-bool recorded() { return at::tracer::impl::is_dispatch_enabled(); }
 
 // False when an operand does not fit the others (the caller then says which)
 // or a trace records, likewise below.

@@ -312,11 +312,18 @@ def decode_step(q: Tensor, k_new: Tensor, v_new: Tensor, k_cache: Tensor, v_cach
     [N,H,D] in q.dtype."""
     flags = _DECODE_NORMS.get(normalize)
     if flags is not None:
-        out = L.host().decode_step(q, k_new, v_new, k_cache, v_cache, pos_in, pos_out, float(scale),
-                                   flags | (L.DECODE_SELF if include_self else 0), tau)
+        args = (q, k_new, v_new, k_cache, v_cache, pos_in, pos_out, float(scale),
+                flags | (L.DECODE_SELF if include_self else 0), tau)
+        out = L.host().decode_step(*args)
         if out is not None:
             return out
-    # refused: say why
+        if torch.jit.is_tracing():  # the registered op, which the trace records
+            return torch.ops.bozo.decode_step(*args)
+    _refuse_decode(q, k_new, v_new, k_cache, v_cache, pos_in, pos_out, tau)
+
+
+def _refuse_decode(q, k_new, v_new, k_cache, v_cache, pos_in, pos_out, tau) -> None:
+    """Say why a step did not run."""
     _on_gpu(q, k_new, v_new, k_cache, v_cache, pos_in, pos_out, tau)
     _check_decode_operands(q, k_new, v_new, k_cache, v_cache, pos_in, pos_out, tau)
     _supported(q, k_new, v_new, k_cache, v_cache, tau)
@@ -524,3 +531,15 @@ def _rope_grad(ctx, dy):
 
 
 _op_rope.register_autograd(_rope_grad, setup_context=_rope_setup)
+
+
+# The decode step while torch.jit.trace records (the native call path sends
+# nothing through the dispatcher but the output's allocation).
+
+@torch.library.custom_op("bozo::decode_step", mutates_args=("k_cache", "v_cache", "pos_out", "tau"), device_types="cuda")
+def _op_decode_step(q: Tensor, k_new: Tensor, v_new: Tensor, k_cache: Tensor, v_cache: Tensor, pos_in: Tensor,
+                    pos_out: Optional[Tensor], scale: float, flags: int, tau: Optional[Tensor]) -> Tensor:
+    out = L.host().decode_step(q, k_new, v_new, k_cache, v_cache, pos_in, pos_out, scale, flags, tau)
+    if out is None:
+        _refuse_decode(q, k_new, v_new, k_cache, v_cache, pos_in, pos_out, tau)
+    return out
