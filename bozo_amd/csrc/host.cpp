@@ -407,6 +407,9 @@ bool paged_append(const Tensor& k, const Tensor& v, const OptTensor& ke, const O
   check(tension_paged_append(&c.c, bk.get(), bv.get(), counter_ptr(st), counter_ptr(ct), N, kn.size(1), kn.size(2),
                              kn.size(3), stream_of(k)),
         "tension_paged_append");
+  // written in place: a graph that saved the pages must see it (inference tensors have no version)
+  for (const Tensor& t : {k, v, opt(ke), opt(ve)})
+    if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
   return true;
 }
 
