@@ -14,6 +14,9 @@ struct FastDiv {
 };
 __device__ __forceinline__ int fdiv(int n, FastDiv d) { return (int)((__umulhi((unsigned)n, d.m) + (unsigned)n) >> d.s); }
 
+// A launch counts its threads in 32 bits.
+inline bool launchable(int64_t workgroups, int64_t threads) { return workgroups * threads <= 0xffffffffll; }
+
 inline FastDiv fast_div(int64_t d) {
   int s = 0;
   while (((int64_t)1 << s) < d) ++s;

@@ -440,6 +440,7 @@ bool launch_vec(const PagedRowsParams& p, hipStream_t st) {
     unsigned n = (unsigned)((g.units + per - 1) / per);
     g.runs = APPEND && n >= 2048;
     n = g.runs ? (n + 63) / 64 * 64 : (n + 7) / 8 * 8;
+    if (!launchable(n, kThreads)) return false;  // the kernel for any rows loops over them
     paged_rows_vec<APPEND, LPR, R, KF32, VF32><<<n, kThreads, 0, st>>>(p, g);
     return true;
   };

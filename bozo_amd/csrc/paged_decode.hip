@@ -161,13 +161,14 @@ void launch_join(const PagedDecodeParams& p, hipStream_t st) {
 // the matrix kernel holds head dim 128), with 128 keys to a split at least.
 void paged_decode_split(int64_t N, int64_t H, int64_t Hk, int64_t D, int64_t keys, int* splits, int* chunk) {
   constexpr float kCuBytesPerUs = 49e3f, kAllBytesPerUs = 23e3f, kJoinUs = 3.5f;
-  constexpr int64_t kLeast = 128;
+  constexpr int64_t kLeast = 128, kMostGroups = ((int64_t)1 << 22) - 1;
   const int64_t rows = N * Hk, cus = device_cus();
   const float row_bytes = (float)keys * (float)(4 * D);
   const float all_us = (float)rows * row_bytes / (kAllBytesPerUs * (float)cus);
   const int fills = H > Hk && D > 64 ? 2 : 4;
   int64_t most = keys / kLeast;
-  if (N * H > 0 && most > ((int64_t)1 << 30) / (N * H)) most = ((int64_t)1 << 30) / (N * H);  // workgroups of a launch
+  // workgroups of a launch, of 1024 threads at most
+  if (N * H > 0 && most > kMostGroups / (N * H)) most = kMostGroups / (N * H);
   float best = 0.f;
   int64_t ns = 1;
   for (int f = 0; f <= fills; ++f) {
@@ -194,7 +195,8 @@ void paged_decode_split(int64_t N, int64_t H, int64_t Hk, int64_t D, int64_t key
 int launch_paged_decode(const PagedDecodeParams& p, hipStream_t st, hipError_t* err) {
   if (!launch_paged_decode_rows(p, st)) {
     const unsigned grid = (unsigned)((int64_t)p.N * p.H * p.splits);
-    if (p.D <= 64) paged_decode_any<4, 16><<<grid, 1024, 0, st>>>(p);
+    if (p.D <= 64 && launchable(grid, 1024)) paged_decode_any<4, 16><<<grid, 1024, 0, st>>>(p);
+    else if (p.D <= 64) paged_decode_any<4, 8><<<grid, 512, 0, st>>>(p);
     else paged_decode_any<16, 8><<<grid, 512, 0, st>>>(p);
   }
   *err = hipGetLastError();
