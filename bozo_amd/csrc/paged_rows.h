@@ -214,7 +214,7 @@ struct Query {
 // PLAIN: the head dim fills a row's lanes, and values and their exponents lie as
 // keys and theirs do.
 template <int KD, int VD, int VPL, int LPR, int G, int U, bool ALIGNED, bool PLAIN>
-__global__ void __launch_bounds__(G == 1 ? 1024 : 512) paged_decode_rows(PagedDecodeParams p, DecodeGrid grid) {
+__global__ void __launch_bounds__(512) paged_decode_rows(PagedDecodeParams p, DecodeGrid grid) {
   constexpr int RPW = 64 / LPR;
   constexpr bool KE = KD == TENSION_E4M3, VE = VD == TENSION_E4M3;
   using PK = Piece<KD, VPL, LPR>;
