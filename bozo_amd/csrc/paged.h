@@ -153,8 +153,9 @@ struct DecodeGrid {
     // (e4m3, N128 H16: W256 17.5 -> 16.2 us, 2000 ragged tokens 62.4 -> 60.5; other pages: the same either way).
     // Where CUs take several workgroups of whole sequences the longest go first, and the next fill of the CUs in
     // reverse, so that each gets its share.  Finding them stands before every load, so only for calls that may read 100
-    // MB (us, in the sequences' order / so: ragged N128 H16 L2000 e4m3 60.4 / 55.9, N32 L4096 float32 114 / 106, N128
-    // L4096 bf16 209.6 / 204; all of one length, N64 H12 L1000 bf16, 32.3 / 32.8).
+    // MB, e4m3 rows counted as they are and others as 16-bit ones (us, in the sequences' order / so: ragged N128 H16 L2000
+    // e4m3 60.4 / 55.9, N32 L4096 float32 114 / 106, N128 L4096 bf16 209.6 / 204; all of one length, N64 H12 L1000 bf16,
+    // 32.3 / 32.8).
     const int64_t cus = device_cus(), per = (int64_t)p.Hk * groups * p.splits;
     const float bytes = (float)p.N * (float)p.Hk * (float)p.most * (float)(p.D * (p.c.ke ? 2 : 4));
     turn = p.W == 0 && p.N > 1 && p.N <= 256 && p.N * per > cus && bytes > 100e6f ? (int)((cus + per - 1) / per) : 0;

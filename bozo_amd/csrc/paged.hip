@@ -1,8 +1,10 @@
 // Paged K/V cache: tokens written into pages (quantised to e4m3 on the way or
 // as they are) and read back dense.  Both are streams: a row of D values is
 // read once and written once, so HBM bounds them (bf16 prompts, 262 MB: 50 us,
-// 5.3 TB/s, what a large copy reaches; e4m3 read back, 303 MB: 65 us), and below
-// some 20 MB the chain of start, table, rows (about 4 us).
+// 5.3 TB/s, what a large copy reaches; e4m3 read back, 303 MB: 62-66 us), and below
+// some 20 MB the chain of start, table, rows (about 4 us).  A read needs that
+// chain; an append's dense rows do not depend on it, but are loaded for tokens
+// that have a place only, so they wait for it too.
 //
 // Quantised rows: with E the biased exponent of a row's largest finite
 // magnitude a and M its mantissa bits, 448 = 1.75 * 2^8 gives the smallest e

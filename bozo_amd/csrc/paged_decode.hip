@@ -40,7 +40,7 @@ __device__ __forceinline__ void bits_to_floats(int dt, const unsigned* w, float*
 // One workgroup per (n, h, split), sixteen lanes to a row, a value at a time:
 // for rows that are no whole pieces of eight values, and pairs of types that
 // have no kernel of their own.  Bound by its loads' number and latency (N16 H12,
-// 1000 keys: bf16 D20 30 us, D100 127; D24 on the kernels for whole pieces 6.2).
+// 1000 keys: bf16 D20 31 us, D100 150; D24 on the kernels for whole pieces 7.3).
 template <int VPL, int kWaves>
 __global__ void __launch_bounds__(64 * kWaves) paged_decode_any(PagedDecodeParams p) {
   constexpr int kRows = 4;
@@ -157,6 +157,9 @@ void launch_join(const PagedDecodeParams& p, hipStream_t st) {
 // of them 23 KB/us each; partial sums and the second kernel cost about 3 us on
 // the card, 4 on the host (bf16 D64, us in one kernel / split: N1 H12 L512 5.5 /
 // 7.2, L1024 9.2 / 7.1, L8192 47 / 10; N16 H12 L1000 10.1 / 12.3, L3000 25 / 28).
+// Rows are counted as 16-bit ones whatever the pages' type: N1 H12 in one kernel
+// / by this rule, 800 keys float32 9.8 / 9.8 (not split, though it would take
+// about 8), 1200 keys e4m3 8.2 / 8.2, float32 13.9 / 8.3; 1700 e4m3 9.9 / 8.3.
 // Tried: one split, and what gives each CU one to four workgroups (two where
 // the matrix kernel holds head dim 128), with 128 keys to a split at least.
 void paged_decode_split(int64_t N, int64_t H, int64_t Hk, int64_t D, int64_t keys, int* splits, int* chunk) {

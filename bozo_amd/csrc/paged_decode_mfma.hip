@@ -14,13 +14,14 @@
 // number; its row's scale is applied to the score, or to tau).  tau enters as
 // three bf16 terms that make up its float32 value; sums are float32.
 //
-// Bound by HBM: 32 keys of 128 e4m3 values (8.3 KB) take a wave about 900 cycles
-// of vector instructions, a quarter of what the card's rate leaves it; the time
-// hardly grows with the heads (bf16 D64, 268 MB, two to eight heads: 43.8 to
-// 46.1 us, 5.8-6.1 TB/s; e4m3 D128, N2, 65500 keys, 135 MB: 25.7 us, 5.3 TB/s).
+// Bound by HBM: vector instructions issue in a quarter of a wave's cycles (e4m3,
+// head dim 128), and the time hardly grows with the heads (two to sixteen: bf16
+// D64, 268 MB, 45-48 us, 5.6-6 TB/s; bf16 D128, 268 MB, 67-69 us; e4m3 D128, N2,
+// 65500 keys, 135 MB: 25.8 us, 5.2 TB/s, 31-32 with the join).  The third term
+// of tau costs e4m3 4% at D64 and 2% at D128, bf16 at most 1%.
 // The next step's K and V are loaded as soon as this step's are operands.
-// Three waves per SIMD for e4m3 at head dim 128 (152 registers); bf16 there
-// keeps two (three spill: 90 -> 101 us).
+// Three waves per SIMD for e4m3 at head dim 128 (158 registers); bf16 there
+// keeps two (three spilled and took 12% longer).
 #include "mfma_common.h"
 #include "paged.h"
 

@@ -15,10 +15,10 @@ namespace {
 bool rows_aligned(const Buf& b) { return row_pieces(b, b.dt == TENSION_E4M3 ? 8 : 16); }
 
 // Waves of a workgroup.  Up to one workgroup per CU the call waits for memory
-// (N16 H12, 1000 bf16 keys: eight waves 10.2 us, four 12.3), and where each
-// takes long the last to end count (N128 H16, up to 4096 ragged: 212 against
-// 219).  Windows of two batches of a pair of waves leave the others nothing
-// (N128 H16 W64 e4m3: two waves 8.3 us, four 10.6).
+// (N16 H12, 1000 bf16 keys: eight waves 11.1 us, four 12.3), and where each
+// takes long the last to end count (N128 H16, up to 4096 ragged bf16 keys, the
+// longest first: 205.5 against 206.7).  Windows of two batches of a pair of
+// waves leave the others nothing (N128 H16 W64 e4m3: two waves 8.5 us, four 10.7).
 int waves_for(const PagedDecodeParams& p) {
   const int64_t groups = (int64_t)p.N * p.Hk * p.splits, cus = device_cus();
   const int64_t keys = p.splits > 1 ? p.chunk : p.most;
@@ -32,8 +32,9 @@ int waves_for(const PagedDecodeParams& p) {
 bool launch_paged_decode_rows(const PagedDecodeParams& p, hipStream_t st) {
   if (p.D % 8 || !rows_aligned(p.c.k) || !rows_aligned(p.c.v)) return false;
   if (!DecodeGrid::fits(p)) return false;
-  // A shared key head on the matrix units where its types allow: two query heads cost the same either way (bf16 D64,
-  // 268 MB: 48 us), four 48.8 against 59.0 us, eight 50 against 102; e4m3 D128, 135 MB, four heads 30 against 50 us.
+  // A shared key head on the matrix units where its types allow (us, against the vector units, of back-to-back calls):
+  // bf16 D64, 268 MB: two query heads 47 / 47, four 47 / 49, eight 47 / 96; e4m3 D128, 135 MB: 30.5 / 33.7, 30.6 / 58,
+  // 31 / 87.
   if (p.H / p.Hk >= 2 && launch_paged_decode_mfma(p, st)) return true;
   const int waves = waves_for(p);
   if (p.c.k.dt == TENSION_F32 && p.c.v.dt == TENSION_BF16) return launch_paged_rows_mixed(p, waves, st);

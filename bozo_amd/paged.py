@@ -45,8 +45,9 @@ class PagedKV(NamedTuple):
     @classmethod
     def empty(cls, pages: int, page_size: int, heads: int, head_dim: int, dtype: torch.dtype = torch.bfloat16,
               v_dtype: Optional[torch.dtype] = None, device="cuda") -> "PagedKV":
-        """Pages that hold nothing yet (their memory is not initialised: no
-        row is read before it is written)."""
+        """Pages that hold nothing yet.  Their memory is not initialised: a
+        position that has a page but was never appended reads back as
+        anything, and so does a length that counts it."""
         both = (dtype, v_dtype or dtype)
         for t in both:
             if t not in _PAGES:
@@ -115,7 +116,8 @@ def paged_append(kv: PagedKV, k_new: Tensor, v_new: Tensor, table: Tensor, start
 
     table: int32 [N, pages per sequence]; start, counts: int32 [N], all on
     the GPU.  Positions that the table has no page for are left out.  The
-    pages that are written must belong to one sequence each."""
+    pages that are written must belong to one sequence each; their version
+    counters are raised, as by any write in place."""
     args = (*kv, k_new, v_new, table, start, counts)
     if L.host().paged_append(*args):
         return
@@ -135,7 +137,8 @@ def _refuse_append(k, v, k_exp, v_exp, k_new, v_new, table, start, counts) -> No
 def paged_read(kv: PagedKV, table: Tensor, start: Tensor, T: int,
                dtype: Union[torch.dtype, tuple, None] = None, counts: Optional[Tensor] = None):
     """Read positions start[n] .. start[n] + T - 1 back: dense K, V
-    [N, T, Hk, D]; zeros past counts[n] and where there is no page.
+    [N, T, Hk, D]; zeros past counts[n] and where there is no page, whatever
+    the page holds where no token was appended.
 
     dtype: of both, or a pair (K's, V's); default the pages' own, bfloat16 for
     float8_e4m3fn (which holds its values exactly)."""

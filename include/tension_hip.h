@@ -400,8 +400,10 @@ int tension_paged_read(const tension_paged* cache, const tension_buf* k_out,
  *   lengths[n] - 1; lo = max(0, lengths[n] - 1 - W), or 0 with W == 0.
  *   out = sum tau v, tau = sigmoid(q . k / scale), divided by max(sum tau,
  *   1e-6) with TENSION_NORM_MASS, by max(hi - lo, 1) with
- *   TENSION_NORM_COUNT; zeros where there is no key.  Rows of keys outside
- *   [lo, hi) are not read.
+ *   TENSION_NORM_COUNT; zeros where there is no key.  Rows outside [lo, hi)
+ *   have no part in the result, whatever they hold, but may be loaded: other
+ *   rows of the pages that the range touches, and the first page for an entry
+ *   that is no page.  So all P pages must be memory that can be read.
  *   max_len: a bound of the lengths that the host knows (0: none); it only
  *   shapes the launch, a longer sequence is attended to in full.
  *   workspace: tension_paged_decode_workspace() bytes for the same sizes
