@@ -291,9 +291,7 @@ def _prepare_reorder(case, g, host, seed):
     else:
         (k, ke), (v, ve) = _pool(g, layers * P, Hk, S, D), _pool(g, layers * P, Hk, S, D)
         tensors = [x.unflatten(0, (layers, P)) for x in (k, v, ke, ve)]
-    # a program has a cache for each layer in hand
-    typed = [t.view(torch.float4_e2m1fn_x2) for t in tensors[:2]] + tensors[2:] if case["pages"] == "e2m1" else tensors
-    return {"case": case, "layers": list(zip(*(t.unbind(0) for t in typed))), "table": table.view(N * B, width).cuda(), "parents": _parents(case, seed).cuda(),
+    return {"case": case, "table": table.view(N * B, width).cuda(), "parents": _parents(case, seed).cuda(),
             "lengths": torch.full((N,), L, dtype=torch.int32).cuda(), "tensors": tensors}
 
 
@@ -487,7 +485,10 @@ def _run_select(s):
 def _run_reorder(s):
     if own:
         import bozo_amd
-        layers = [bozo_amd.PagedKV(*t) for t in s["layers"]]
+        tensors = s["tensors"]
+        if s["case"]["pages"] == "e2m1":
+            tensors = [t.view(torch.float4_e2m1fn_x2) for t in tensors[:2]] + tensors[2:]
+        layers = [bozo_amd.PagedKV(*(t[i] for t in tensors)) for i in range(s["case"]["layers"])]
         table = bozo_amd.paged_reorder(layers, s["table"], s["lengths"], s["parents"])
     else:
         table = _plain_reorder(s)
