@@ -2,7 +2,7 @@
 //   score(b, v) = scores[b] + x[b, v] - log sum_u exp x[b, u],
 // the K largest of a group, the lower of b * V + v where two are equal.
 //
-// Logarithm and sum are taken in 64 bits, since they decide between beams:
+// Exponentials, sum and logarithm are taken in 64 bits, since they decide between beams:
 // within a beam the logits' own order is the scores', so a beam's candidates
 // are found by comparing what was stored, and only they get a score.
 #include <float.h>
@@ -42,23 +42,32 @@ __device__ __forceinline__ uint64_t wave_most(uint64_t x) {
   return x;
 }
 
-// 2^u for -1000 <= u <= 0, to 4e-11 relative: 2^round(u) times a polynomial of the
-// rest on [-1/2, 1/2] (least greatest relative error, fitted by reweighted least
-// squares).  Adding 1.5 * 2^52 rounds, and leaves round(u) in the low bits.
-__device__ __forceinline__ double exp2_below(double u) {
+constexpr int kPowers = 64;
+
+// 2^(j / 64), for add_exp: made by each workgroup, 1 exactly at 0.
+__device__ __forceinline__ void make_powers(double* powers) {
+  if (threadIdx.x < kPowers) powers[threadIdx.x] = exp2((double)threadIdx.x / kPowers);
+}
+
+// s + exp(d) for d <= 0 in 64 bits; exp(0) is 1 exactly, so that a beam's only
+// token adds nothing to its score (what is below 2^-1000 counts as that).  With u =
+// 64 d log2 e = 64 k + j + f, |f| <= 1/2: 2^k 2^(j / 64) times 1 + f q(f), where q
+// interpolates (2^(f / 64) - 1) / f at Chebyshev points (2^-58 relative, below the
+// roundings).  Adding 1.5 * 2^52 rounds, and leaves 64 k + j in the low bits.
+__device__ __forceinline__ double add_exp(double s, double d, const double* powers) {
   constexpr double kRound = 6755399441055744.;
+  const double u = fmax(d * (kPowers * kLog2e64), -1000. * kPowers);
   const double t = u + kRound;
   const double f = u - (t - kRound);
-  double p = 1.5201921656720236e-05;
-  p = __builtin_fma(p, f, 0.00015469291292481165);
-  p = __builtin_fma(p, f, 0.0013333922564639832);
-  p = __builtin_fma(p, f, 0.0096180272532031662);
-  p = __builtin_fma(p, f, 0.0555041035344494);
-  p = __builtin_fma(p, f, 0.24022651198160949);
-  p = __builtin_fma(p, f, 0.69314718072844861);
-  p = __builtin_fma(p, f, 0.99999999996168187);
-  const uint64_t n = __builtin_bit_cast(uint64_t, t), b = __builtin_bit_cast(uint64_t, p);
-  return __builtin_bit_cast(double, b + (n << 52));
+  double p = 0.001333356978334557 / (64. * 64. * 64. * 64. * 64.);
+  p = __builtin_fma(p, f, 0.009618140859595685 / (64. * 64. * 64. * 64.));
+  p = __builtin_fma(p, f, 0.055504108664803826 / (64. * 64. * 64.));
+  p = __builtin_fma(p, f, 0.2402265069589214 / (64. * 64.));
+  p = __builtin_fma(p, f, 0.6931471805599453 / 64.);
+  p = __builtin_fma(p, f, 1.);
+  const int n = (int)(unsigned)__builtin_bit_cast(uint64_t, t);
+  const uint64_t b = __builtin_bit_cast(uint64_t, powers[n & (kPowers - 1)]);
+  return __builtin_fma(__builtin_bit_cast(double, b + ((uint64_t)(unsigned)(n >> 6) << 52)), p, s);
 }
 
 template <int CTRL>
@@ -128,9 +137,12 @@ constexpr int kPer = kSpan / kThreads, kMost = 1024;
 // on each thread is a group), which are put in order by counting what is before
 // each.  Where more than kMost do (equal logits) they are taken out one by one.
 //
-// Bound by the sums in 64 bits, sixteen of about 24 instructions a logit (10 us of
-// issue for 512 rows of 32768 bf16 logits), and HBM: 17.5 us there, 1.9 TB/s.
-// Sums of float32 exponentials took 21, halved spans or twice the threads more.
+// 512 rows of 32768 bf16 logits: 18.4 us in a trace, 1.8 TB/s.  No one thing bounds
+// it: loads, maximum, bound, sums (19 instructions a logit, fourteen of them on 64
+// bits: 8 us of issue) and order follow each other in a workgroup, and five waves
+// a SIMD hide a part of each.  Exponentials without the table, by a polynomial of
+// degree 11, took 0.9 us more, float32 ones 3.5, halved spans or twice the threads
+// more as well.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) beam_spans(BeamParams p) {
   constexpr int kVec = 16 / sizeof(T);
@@ -139,6 +151,7 @@ __global__ void __launch_bounds__(kThreads) beam_spans(BeamParams p) {
   __shared__ float group[kThreads], top[kThreads / 64];
   __shared__ double sums[kThreads / 64];
   __shared__ uint64_t best[kThreads / 64];
+  __shared__ double powers[kPowers];
   __shared__ int count;
   const int span = blockIdx.x % p.spans, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int row = blockIdx.x / p.spans, n = row / p.B, b = row % p.B;
@@ -171,6 +184,7 @@ __global__ void __launch_bounds__(kThreads) beam_spans(BeamParams p) {
       }
     }
   }
+  make_powers(powers);
   if (tid == 0) count = 0;
   float own = -INFINITY;
 #pragma unroll
@@ -213,7 +227,7 @@ __global__ void __launch_bounds__(kThreads) beam_spans(BeamParams p) {
 
   double s = 0.;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) s += exp2_below(fmax(((double)x[i] - (double)most) * kLog2e64, -1000.));
+  for (int i = 0; i < kPer; ++i) s = add_exp(s, (double)x[i] - (double)most, powers);
   s = wave_sum(s);
   if (lane == 0) sums[wave] = s;
   __syncthreads();
@@ -268,7 +282,7 @@ __device__ __forceinline__ void beam_base_of(const BeamParams& p, float score, b
     if (WAVE) most = wave_max(most);
     for (int i = first; i < p.spans; i += step) {
       const double d = ((double)s[i].most - (double)most) * kLog2e64;
-      sum += s[i].most > -INFINITY ? s[i].sum * exp2_below(fmax(d, -1000.)) : 0.;
+      sum += s[i].most > -INFINITY ? s[i].sum * exp2(d) : 0.;
     }
     if (WAVE) sum = wave_sum(sum);
   }
@@ -353,6 +367,7 @@ __global__ void __launch_bounds__(64 * kFewBeams) beam_few(BeamParams p, GroupGe
   __shared__ Candidate found[kCandidates];
   __shared__ Candidate best[kFewBeams];
   __shared__ float head[kFewBeams][64];
+  __shared__ double powers[kPowers];
   __shared__ int count;
   const int n = blockIdx.x, tid = threadIdx.x, lane = tid & 63, b = __builtin_amdgcn_readfirstlane(tid >> 6);
   const T* x0 = (const T*)p.x.p + (n * p.x.s0 + b * p.x.s1);
@@ -372,7 +387,9 @@ __global__ void __launch_bounds__(64 * kFewBeams) beam_few(BeamParams p, GroupGe
       for (int j = 0; j < kVec; ++j) x[i + j] = v + j < p.V ? (float)x0[v + j] : -INFINITY;
     }
   }
+  make_powers(powers);
   if (tid == 0) count = 0;
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < kOwn; ++i) own = __builtin_elementwise_maximum(own, x[i]);  // a NaN stays one
   const float most = wave_max(own);
@@ -381,7 +398,7 @@ __global__ void __launch_bounds__(64 * kFewBeams) beam_few(BeamParams p, GroupGe
   if (reads) {
     double s = 0.;
 #pragma unroll
-    for (int i = 0; i < kOwn; ++i) s += exp2_below(fmax(((double)x[i] - (double)most) * kLog2e64, -1000.));
+    for (int i = 0; i < kOwn; ++i) s = add_exp(s, (double)x[i] - (double)most, powers);
     base -= log(wave_sum(s));
   }
   const Candidate end = {live && ended && lane == 0 ? base : -INFINITY, (unsigned)(b * p.V + (int)p.pad)};

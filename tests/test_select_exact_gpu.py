@@ -1,0 +1,99 @@
+"""Scores of beam selection to 64 bits: what the definition settles exactly comes
+out so, in one launch, over spans, and over many lists."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from bozo_amd import beam_select
+from oracle import serving_ref as R
+
+pytestmark = pytest.mark.gpu
+
+# B, V, K: one launch, one and several spans of a vocabulary, many lists
+SIZES = [(2, 1, 1), (2, 7, 2), (4, 2048, 4), (16, 2000, 32), (2, 2049, 2), (4, 20000, 16), (17, 300, 8), (64, 20000, 64), (40, 9000, 50)]
+
+
+def select(x, s, K, ended=None, pad=0):
+    out = beam_select(x, s, K, ended=ended, pad=pad)
+    want = R.select(x.float().cpu().numpy(), s.cpu().numpy(), K, None if ended is None else ended.cpu().numpy(), pad)
+    return [t.cpu().numpy() for t in out], want
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,V,K", SIZES)
+def test_one_live_token_has_log_probability_zero(B, V, K, dt):
+    """A beam with one token above -inf, wherever it lies and whatever its logit: its score is the beam's."""
+    x = torch.full((3, B, V), -math.inf, device="cuda", dtype=dt)
+    for n in range(3):
+        for b in range(B):
+            x[n, b, (n * 977 + b * 8191) % V] = (b - 3) * 7.5 * (n + 1)
+    s = torch.zeros(3, B, device="cuda")
+    s[1] = -torch.arange(B, device="cuda") * 0.37
+    s[2] = -1.0
+    (out, tok, par), (want, wt, wp) = select(x, s, K)
+    assert np.array_equal(out, want.astype(np.float32)) and np.array_equal(tok, wt) and np.array_equal(par, wp)
+    assert np.array_equal(out[0, :min(B, K)], np.zeros(min(B, K), np.float32))
+
+
+@pytest.mark.parametrize("ended_first", [True, False])
+@pytest.mark.parametrize("B,V,K", SIZES)
+def test_ended_and_forced_beams_tie(B, V, K, ended_first):
+    """An ended beam and one whose next token is certain, of one score: the lower place first, with one kept too."""
+    x = torch.full((1, B, V), -math.inf, device="cuda")
+    x[:, :, V - 1] = 3.25
+    ended = torch.zeros(1, B, dtype=torch.bool, device="cuda")
+    ended[:, (0 if ended_first else 1)::2] = True
+    s = torch.full((1, B), -1.0, device="cuda")
+    for k in sorted({1, min(2, B * V), K}):
+        (out, tok, par), (want, wt, wp) = select(x, s, k, ended, V // 2)
+        assert np.array_equal(tok, wt) and np.array_equal(par, wp) and np.array_equal(out, want.astype(np.float32)), k
+        assert par[0, 0] == 0 and tok[0, 0] == (V // 2 if ended_first else V - 1)
+
+
+@pytest.mark.parametrize("B,V,K", [c for c in SIZES if c[1] > 1])
+def test_scores_to_64_bits(B, V, K):
+    """Log probabilities that are nothing but a small sum, and ordinary ones.
+
+    A sum's exponentials are off by 2^-52 of their exponents (ln V of them on the whole, 14 at most), 2^-51 of their own
+    and 2^-47 by their order, its logarithm by that and 2^-50 of itself, the oracle's likewise: 2^-45 covers both.  Then one rounding."""
+    g = torch.Generator(device="cuda").manual_seed(V)
+    near = -24 - 6 * torch.rand(2, B, V, generator=g, device="cuda")
+    near[:, :, V // 3] = 0.0
+    wide = torch.randn(2, B, V, generator=g, device="cuda") * 3
+    for x in (near, wide):
+        for score in (0.0, -2.5):
+            s = torch.full((2, B), score, device="cuda")
+            (out, tok, par), _ = select(x, s, K)
+            full = {}
+            y = x.double().cpu().numpy()
+            c = score + y - y.max(-1, keepdims=True) - np.log(np.exp(y - y.max(-1, keepdims=True)).sum(-1, keepdims=True))
+            for n in range(2):
+                want = c[n, par[n], tok[n]]
+                assert (np.abs(out[n] - want) <= 2.0 ** -24 * np.abs(want) + 2.0 ** -45).all()
+                assert (np.diff(want) <= 2.0 ** -45).all()
+                assert want[-1] >= np.sort(c[n].ravel())[-K] - 2.0 ** -45
+
+
+@pytest.mark.parametrize("B,V", [(2, 2000), (2, 20000), (64, 20000)])
+def test_beams_that_are_close(B, V):
+    """Gaps far below a float32's step of the sum of exponentials, far above its 64-bit error: the order is theirs."""
+    g = torch.Generator(device="cuda").manual_seed(V)
+    x = -22 - 4 * torch.rand(1, 1, V, generator=g, device="cuda").expand(1, B, V).contiguous()
+    x[:, :, 5] = 0.0
+    y = x[0, 0].double().cpu().numpy()
+    own = -np.log(np.exp(y).sum())  # of beam 1, some 1e-6
+    ended = torch.ones(1, B, dtype=torch.bool, device="cuda")
+    ended[0, 1] = False
+    for k in range(-30, 31):
+        other = np.float32(own)
+        for _ in range(abs(k)):
+            other = np.nextafter(other, np.float32(-1 if k < 0 else 1))
+        if abs(float(other) - own) < 2.0 ** -44:
+            continue
+        s = torch.full((1, B), -5.0, device="cuda")
+        s[0, 0], s[0, 1] = float(other), 0.0
+        (out, tok, par), _ = select(x, s, 2, ended, 9)
+        assert par[0].tolist() == ([0, 1] if other > own else [1, 0]), (k, float(other), own)
+        assert tok[0].tolist() == ([9, 5] if other > own else [5, 9])
