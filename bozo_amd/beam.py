@@ -29,8 +29,10 @@ def beam_select(logits: Tensor, scores: Tensor, count: Optional[int] = None, *, 
 
         scores[n, b] + log_softmax(logits[n, b])[v],
 
-    taken in 64 bits and rounded once; of equal ones the lower b * V + v comes
-    first, and within a beam the logits' order is the scores'.  ended (bool or
+    taken in 64 bits and rounded once.  Of equal ones the lower beam's come first;
+    within a beam the logits decide, the lower token of equal ones, also where
+    scores do not tell them apart.  (Beams within about 1e-14 of each other are
+    as near as sums in 64 bits are.)  ended (bool or
     uint8 [N, B]): a beam at its end has one continuation, token ``pad`` with the
     score it has.  A beam whose logits hold a NaN or +inf or nothing above -inf,
     or whose score is NaN or +inf, has none; where fewer than ``count`` are left,

@@ -1,10 +1,12 @@
 // The best continuations of a group's beams over the vocabulary:
 //   score(b, v) = scores[b] + x[b, v] - log sum_u exp x[b, u],
-// the K largest of a group, the lower of b * V + v where two are equal.
+// the K largest of a group; of equal ones the lower beam's, within a beam the
+// larger logit, then the lower token.
 //
-// Exponentials, sum and logarithm are taken in 64 bits, since they decide between beams:
-// within a beam the logits' own order is the scores', so a beam's candidates
-// are found by comparing what was stored, and only they get a score.
+// Exponentials, sum and logarithm are taken in 64 bits, since they decide between
+// beams.  Within a beam the logits' own order is the scores', also where scores
+// round to one, so a beam's candidates are found by comparing what was stored, and
+// only they get a score.
 #include <float.h>
 
 #include "paged.h"
@@ -27,7 +29,6 @@ __device__ __forceinline__ float key_logit(uint64_t k) {
   const unsigned o = (unsigned)(k >> 32);
   return __builtin_bit_cast(float, o & 0x80000000u ? o & 0x7fffffffu : ~o);
 }
-__device__ __forceinline__ unsigned key_index(uint64_t k) { return 0xffffffffu - (unsigned)k; }
 
 __device__ __forceinline__ uint64_t shfl64(uint64_t x, int from) {
   const unsigned lo = (unsigned)__shfl((int)(unsigned)x, from), hi = (unsigned)__shfl((int)(x >> 32), from);
@@ -291,14 +292,22 @@ __device__ __forceinline__ void beam_base_of(const BeamParams& p, float score, b
   *base_out = some ? (double)score - (ended ? 0. : log(sum)) : -INFINITY;
 }
 
-// A candidate: its score and its place b * V + v in the group.
+// A candidate: its score, and what decides between equal ones as one number, the
+// larger first: 63 - b, the logit's order, 2^20 - 1 - v; 0 behind every candidate.
 struct Candidate {
   double c;
-  unsigned flat;
+  uint64_t rank;
 };
 __device__ __forceinline__ bool before(const Candidate& a, const Candidate& b) {
-  return a.c > b.c || (a.c == b.c && a.flat < b.flat);
+  return a.c > b.c || (a.c == b.c && a.rank > b.rank);
 }
+__device__ __forceinline__ uint64_t rank_of(int b, uint64_t key) {
+  return (uint64_t)(63 - b) << 52 | key >> 32 << 20 | (key & 0xfffff);
+}
+// Of a beam at its end, whose only candidate is token `pad`.
+__device__ __forceinline__ uint64_t rank_of_end(const BeamParams& p, int b) { return rank_of(b, 0xffffffffu - (unsigned)p.pad); }
+__device__ __forceinline__ int rank_beam(uint64_t rank) { return 63 - (int)(rank >> 52); }
+__device__ __forceinline__ int rank_token(uint64_t rank) { return 0xfffff - (int)(rank & 0xfffff); }
 
 constexpr int kCandidates = 2048, kLists = 512;  // of a group that beam_groups takes
 constexpr int kEach = kCandidates / kThreads, kManyThreads = 1024;
@@ -308,12 +317,14 @@ struct GroupGeometry {
   int each, ranks;  // of beam_groups_many: threads to a list, ranks that give the bound
 };
 
-__device__ __forceinline__ void put(const BeamParams& p, const GroupGeometry& g, int k, double c, unsigned flat) {
+__device__ __forceinline__ void put(const BeamParams& p, int k, double c, int b, int v) {
   const int64_t o = (int64_t)blockIdx.x * p.K + k;
-  const int b = fdiv((int)flat, g.vocabulary);
   p.out[o] = (float)c;
-  p.tokens[o] = (int)flat - b * p.V;
+  p.tokens[o] = v;
   p.parents[o] = b;
+}
+__device__ __forceinline__ void put(const BeamParams& p, int k, const Candidate& x) {
+  put(p, k, x.c, rank_beam(x.rank), rank_token(x.rank));
 }
 
 // The K best of `some` candidates, which hold them, by counting what is before each.
@@ -325,14 +336,15 @@ __device__ __forceinline__ void put_best(const BeamParams& p, const GroupGeometr
     int ahead = 0;
 #pragma unroll 8
     for (int j = 0; j < some; ++j) ahead += before(found[j], mine);
-    if (ahead < p.K) put(p, g, ahead, mine.c, mine.flat);
+    if (ahead < p.K) put(p, ahead, mine);
   }
   if (some < p.K && tid < 64) {  // no more candidates: the lowest places that were not taken
     bool taken = tid >= p.K;
-    for (int j = 0; j < some; ++j) taken |= found[j].flat == (unsigned)tid;
+    for (int j = 0; j < some; ++j) taken |= rank_beam(found[j].rank) * p.V + rank_token(found[j].rank) == tid;
     const uint64_t free = __ballot(!taken);
     const int k = some + __popcll(free & ((1ull << tid) - 1));
-    if (!taken && k < p.K) put(p, g, k, -INFINITY, tid);
+    const int b = fdiv(tid, g.vocabulary);
+    if (!taken && k < p.K) put(p, k, -INFINITY, b, tid - b * p.V);
   }
 }
 
@@ -340,7 +352,7 @@ __device__ __forceinline__ void put_best(const BeamParams& p, const GroupGeometr
 __device__ __forceinline__ Candidate best_of_block(Candidate mine, Candidate* best, int waves) {
 #pragma unroll
   for (int m = 32; m; m >>= 1) {
-    const Candidate o = {__shfl_xor(mine.c, m), (unsigned)__shfl_xor((int)mine.flat, m)};
+    const Candidate o = {__shfl_xor(mine.c, m), shfl64(mine.rank, (threadIdx.x & 63) ^ m)};
     mine = before(o, mine) ? o : mine;
   }
   if ((threadIdx.x & 63) == 0) best[threadIdx.x >> 6] = mine;
@@ -401,7 +413,7 @@ __global__ void __launch_bounds__(64 * kFewBeams) beam_few(BeamParams p, GroupGe
     for (int i = 0; i < kOwn; ++i) s = add_exp(s, (double)x[i] - (double)most, powers);
     base -= log(wave_sum(s));
   }
-  const Candidate end = {live && ended && lane == 0 ? base : -INFINITY, (unsigned)(b * p.V + (int)p.pad)};
+  const Candidate end = {live && ended && lane == 0 ? base : -INFINITY, rank_of_end(p, b)};
   head[b][lane] = reads ? (float)((double)own - (double)most + base) : (float)end.c;
   __syncthreads();
   float of_set = -INFINITY;
@@ -412,7 +424,7 @@ __global__ void __launch_bounds__(64 * kFewBeams) beam_few(BeamParams p, GroupGe
     if (reads) {
 #pragma unroll
       for (int i = 0; i < kOwn; ++i)
-        if (x[i] > -INFINITY) f(Candidate{(double)x[i] - (double)most + base, (unsigned)(b * p.V + index(i))});
+        if (x[i] > -INFINITY) f(Candidate{(double)x[i] - (double)most + base, rank_of(b, order_key(x[i], (unsigned)index(i)))});
     } else if (end.c > -INFINITY) {
       f(end);
     }
@@ -429,12 +441,12 @@ __global__ void __launch_bounds__(64 * kFewBeams) beam_few(BeamParams p, GroupGe
   }
   Candidate last = {INFINITY, 0};
   for (int k = 0; k < p.K; ++k) {  // equal scores: the best is taken out K times
-    Candidate mine = {-INFINITY, 0xffffffffu};
+    Candidate mine = {-INFINITY, 0};
     each([&](Candidate c) {
       if (before(last, c) && before(c, mine)) mine = c;
     });
     last = best_of_block(mine, best, p.B);
-    if (tid == 0) put(p, g, k, last.c, last.flat);
+    if (tid == 0) put(p, k, last);
   }
 }
 
@@ -473,13 +485,13 @@ __global__ void __launch_bounds__(kThreads) beam_groups(BeamParams p, GroupGeome
   Candidate cand[kEach];
 #pragma unroll
   for (int j = 0; j < kEach; ++j) {
-    cand[j] = Candidate{-INFINITY, 0xffffffffu};
+    cand[j] = Candidate{-INFINITY, 0};
     if (tid + j * kThreads >= all) continue;
     const int b = fdiv(list[j], g.spans);
     if (most[b] == INFINITY) {  // at its end: goes on as it is, once
-      if (rank[j] == 0 && list[j] == b * p.spans) cand[j] = Candidate{base[b], (unsigned)(b * p.V + (int)p.pad)};
+      if (rank[j] == 0 && list[j] == b * p.spans) cand[j] = Candidate{base[b], rank_of_end(p, b)};
     } else if (key[j]) {
-      cand[j] = Candidate{(double)key_logit(key[j]) - most[b] + base[b], (unsigned)b * p.V + key_index(key[j])};
+      cand[j] = Candidate{(double)key_logit(key[j]) - most[b] + base[b], rank_of(b, key[j])};
     }
     if (!(cand[j].c > -INFINITY)) cand[j].c = -INFINITY;  // of a beam that has none
     if (cand[j].c > -INFINITY) atomicMax(&group[(list[j] + 13 * rank[j]) & 63], order_bits((float)cand[j].c));
@@ -525,7 +537,7 @@ __global__ void __launch_bounds__(kManyThreads) beam_groups_many(BeamParams p, G
       const double largest = most[b], add = base[b];
       if (!(add > -INFINITY)) continue;
       if (largest == INFINITY) {  // at its end: goes on as it is, once
-        if (sub == 0 && l == b * p.spans) f(Candidate{add, (unsigned)(b * p.V + (int)p.pad)}, l);
+        if (sub == 0 && l == b * p.spans) f(Candidate{add, rank_of_end(p, b)}, l);
         continue;
       }
       bool on = true;
@@ -540,8 +552,7 @@ __global__ void __launch_bounds__(kManyThreads) beam_groups_many(BeamParams p, G
         for (int j = 0; j < kDeep; ++j) {
           on = on && key[j];
           if (on)
-            on = f(Candidate{(double)key_logit(key[j]) - largest + add, (unsigned)b * p.V + key_index(key[j])},
-                   l + 13 * (r0 + j * g.each));
+            on = f(Candidate{(double)key_logit(key[j]) - largest + add, rank_of(b, key[j])}, l + 13 * (r0 + j * g.each));
         }
       }
     }
@@ -568,13 +579,13 @@ __global__ void __launch_bounds__(kManyThreads) beam_groups_many(BeamParams p, G
   }
   Candidate last = {INFINITY, 0};
   for (int k = 0; k < p.K; ++k) {
-    Candidate mine = {-INFINITY, 0xffffffffu};
+    Candidate mine = {-INFINITY, 0};
     walk(p.K, [&](Candidate x, int) {
       if (before(last, x) && before(x, mine)) mine = x;
       return true;
     });
     mine = best_of_block(mine, best, kWaves);
-    if (tid == 0) put(p, g, k, mine.c, mine.flat);
+    if (tid == 0) put(p, k, mine);
     last = mine;
   }
 }

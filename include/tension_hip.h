@@ -499,8 +499,9 @@ int tension_paged_reorder(const tension_paged* layers, int32_t count,
  *   ended: TENSION_U8 [N,B] (s[0..1]) or NULL; a beam with a byte other than 0
  *     has one continuation, token `pad` with the score it has.
  *   score(b, v) = scores[b] + x[b, v] - log sum_u exp x[b, u], taken in 64 bits.
- *   Larger ones come first, of equal ones the lower b * V + v; within a beam the
- *   order is that of its logits.  A beam whose score is not below infinity or no
+ *   Larger ones come first, of equal ones the lower b; within a beam the order is
+ *   that of its logits, then the lower v, also where scores round to one.  Sums of
+ *   beams are good to about 1e-14.  A beam whose score is not below infinity or no
  *   number, or whose logits hold a NaN or +infinity or nothing above -infinity,
  *   has none but scores of -infinity.  Where fewer than K are above that, the
  *   lowest places that are not taken follow, with -infinity.

@@ -101,11 +101,12 @@ def reorder(table: np.ndarray, lengths, parents: np.ndarray, S: int, P: int):
 
 
 def select(logits: np.ndarray, scores: np.ndarray, K: int, ended=None, pad: int = 0):
-    """(scores float64, tokens, parents) [N, K]."""
+    """(scores float64, tokens, parents) [N, K]; of equal scores the lower beam's first, within a beam the larger
+    logit's, then the lower token."""
     N, B, V = logits.shape
     out, tok, par = np.zeros((N, K)), np.zeros((N, K), np.int64), np.zeros((N, K), np.int64)
     for n in range(N):
-        c = np.full((B, V), -np.inf)
+        c, order = np.full((B, V), -np.inf), np.zeros((B, V))
         for b in range(B):
             s = float(scores[n, b])
             if not (s > -np.inf and s < np.inf):
@@ -118,6 +119,8 @@ def select(logits: np.ndarray, scores: np.ndarray, K: int, ended=None, pad: int 
                 continue
             m = x.max()
             c[b] = s + (x - m - np.log(np.exp(x - m).sum()))
-        at = np.argsort(-c.ravel(), kind="stable")[:K]
+            order[b] = np.where(x > -np.inf, x, 0.0)
+        beam = np.repeat(np.arange(B), V)
+        at = np.lexsort((-order.ravel(), beam, -c.ravel()))[:K]
         out[n], tok[n], par[n] = c.ravel()[at], at % V, at // V
     return out, tok, par

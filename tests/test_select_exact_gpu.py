@@ -97,3 +97,24 @@ def test_beams_that_are_close(B, V):
         (out, tok, par), _ = select(x, s, 2, ended, 9)
         assert par[0].tolist() == ([0, 1] if other > own else [1, 0]), (k, float(other), own)
         assert tok[0].tolist() == ([9, 5] if other > own else [5, 9])
+
+
+@pytest.mark.parametrize("B,V,K", [(1, 2048, 4), (1, 2049, 4), (3, 2048, 32), (3, 2049, 32), (4, 20000, 16), (5, 300, 64), (64, 20000, 64),
+                                   (17, 1000, 33), (1, 1 << 20, 64)])
+def test_logits_that_scores_do_not_tell_apart(B, V, K):
+    """Within a beam the order is the logits', also where a score rounds away what they differ by: on every path."""
+    g = torch.Generator(device="cuda").manual_seed(V + B)
+    x = 1e-17 * torch.randn(2, B, V, generator=g, device="cuda")  # against a logarithm of ln V
+    s = torch.zeros(2, B, device="cuda")
+    x[1], s[1] = x[1] * 1e9, -1e9
+    x[1, 1:] = -math.inf
+    x[1, :, V // 2:] = x[1, :, :V - V // 2].clone()  # and logits that are equal
+    (out, tok, par), (want, wt, wp) = select(x, s, K)
+    assert np.array_equal(tok, wt) and np.array_equal(par, wp)
+    assert np.array_equal(np.sort(-x[0, 0].cpu().numpy())[:min(K, V)], -x[0, 0].cpu().numpy()[tok[0]][:min(K, V)])
+    y = torch.randn(1, B, V, generator=g, device="cuda").bfloat16()  # one beam, whose score leaves steps of 2 or more
+    s = torch.full((1, B), -math.inf, device="cuda")
+    s[0, B // 2] = -1e16
+    (out, tok, par), _ = select(y, s, min(K, V))
+    want = np.lexsort((np.arange(V), -y[0, B // 2].double().cpu().numpy()))[:min(K, V)]
+    assert (par == B // 2).all() and np.array_equal(tok[0], want)
