@@ -20,8 +20,9 @@
 // of the next looked up while one is added up.
 //
 // Roundings: codes become bf16 with their exponents, exactly; a query enters as
-// it is, as two bf16 terms (f16) or as three (float32), tau as three bf16 terms
-// that make up its float32 value; sums are float32.
+// it is, as two bf16 terms (f16) or as three (float32: all of a value's bits, if it
+// is within 2^94 of the row's largest), tau as three bf16 terms that make up its
+// float32 value; sums are float32.
 #include "fp4.h"
 #include "mfma_common.h"
 #include "paged.h"
@@ -56,45 +57,34 @@ __device__ __forceinline__ unsigned halves(unsigned a, unsigned b) {
   return __builtin_amdgcn_perm(b, a, HI ? 0x07060302u : 0x05040100u);
 }
 
-// Eight values of a query row as NQ operands: bf16 terms that make them up, each
-// but the last the leading eight bits of what is left.
-template <int QT, int NQ>
-__device__ __forceinline__ void query_terms(const Buf& q, int64_t off, bool whole, u32x4* term) {
-  if constexpr (QT == TENSION_BF16) {
-    const unsigned short* s = (const unsigned short*)q.p + off;
-    if (whole) {
-      term[0] = *(const u32x4*)s;
-    } else {
+// Eight values of a query row as a bf16 operand.
+__device__ __forceinline__ u32x4 query_bf16(const Buf& q, int64_t off, bool whole) {
+  const unsigned short* s = (const unsigned short*)q.p + off;
+  if (whole) return *(const u32x4*)s;
+  u32x4 x;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) term[0][j] = s[2 * j] | (unsigned)s[2 * j + 1] << 16;
-    }
-  } else {
-    float x[8];
-    if constexpr (QT == TENSION_F16) {
-      const f16* s = (const f16*)q.p + off;
+  for (int j = 0; j < 4; ++j) x[j] = s[2 * j] | (unsigned)s[2 * j + 1] << 16;
+  return x;
+}
+// Eight values as NQ operands: bf16 terms that make them up, each but the last
+// the leading eight bits of what is left.
+template <int NQ>
+__device__ __forceinline__ void query_terms(float* x, u32x4* term) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = (float)s[j];
-    } else {
-      const float* s = (const float*)q.p + off;
+  for (int i = 0; i < NQ; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = s[j];
-    }
+    for (int j = 0; j < 4; ++j) {
+      unsigned w[2];
 #pragma unroll
-    for (int i = 0; i < NQ; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        unsigned w[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float y = x[2 * j + e];
-          w[e] = y == y ? __builtin_bit_cast(unsigned, y) & 0xffff0000u : 0x7fc00000u;
-          const float left = y - __builtin_bit_cast(float, w[e]);
-          // an infinity or a NaN is its first term's alone
-          x[2 * j + e] = left == left ? left : 0.f;
-        }
-        term[i][j] = halves<true>(w[0], w[1]);
+      for (int e = 0; e < 2; ++e) {
+        const float y = x[2 * j + e];
+        w[e] = y == y ? __builtin_bit_cast(unsigned, y) & 0xffff0000u : 0x7fc00000u;
+        const float left = y - __builtin_bit_cast(float, w[e]);
+        // an infinity or a NaN is its first term's alone
+        x[2 * j + e] = left == left ? left : 0.f;
       }
-  }
+      term[i][j] = halves<true>(w[0], w[1]);
+    }
 }
 
 // Which bytes of word w belong to row i, of four rows of G exponents each.
@@ -133,7 +123,7 @@ __global__ void __launch_bounds__(64 * kWaves) fp4_decode_mfma(PagedDecodeParams
   // Rotates the exponent of the lane's piece among its row's to where a scale operand has it; what else the word holds
   // falls on mantissa and sign, which the conversion does not take.
   const int vturn = c * KS / 16 * 8 + 9;
-  const float scale = -p.inv_scale * kLog2e;
+  float scale = -p.inv_scale * kLog2e;
 
   struct Places {
     int id[2], row[2];
@@ -295,9 +285,42 @@ __global__ void __launch_bounds__(64 * kWaves) fp4_decode_mfma(PagedDecodeParams
     {
       const bool whole = ((uintptr_t)p.q.p | (uintptr_t)(p.q.s0 * 2) | (uintptr_t)(p.q.s1 * 2)) % 16 == 0;
       const int64_t off = (int64_t)n * p.q.s0 + (int64_t)(h0 + (c < nh ? c : 0)) * p.q.s1;
+      auto piece = [&](int i) { return off + (i < KS ? g * (W / 4) + 8 * i : W + 8 * g); };
+      if constexpr (QT == TENSION_BF16) {
 #pragma unroll
-      for (int i = 0; i < KS; ++i) query_terms<QT, NQ>(p.q, off + g * (W / 4) + 8 * i, whole, q[i]);
-      if constexpr (kTail) query_terms<QT, NQ>(p.q, off + W + 8 * g, whole, q[KS]);
+        for (int i = 0; i < G; ++i) q[i][0] = query_bf16(p.q, piece(i), whole);
+      } else {
+        float x[G][8];
+#pragma unroll
+        for (int i = 0; i < G; ++i)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[i][j] = QT == TENSION_F16 ? (float)((const f16*)p.q.p)[piece(i) + j] : ((const float*)p.q.p)[piece(i) + j];
+        if constexpr (QT == TENSION_F32) {
+          // A bf16 ends at 2^-133: a row whose values are all small is brought up to 2^-16, and its scores down again.
+          unsigned top = 0;
+#pragma unroll
+          for (int i = 0; i < G; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const unsigned b = magnitude_bits(x[i][j]);
+              top = b > top ? b : top;
+            }
+#pragma unroll
+          for (int m = 16; m < 64; m *= 2) {
+            const unsigned o = (unsigned)__shfl_xor((int)top, m);
+            top = o > top ? o : top;
+          }
+          const int turn = top >> 23 < 111 ? 111 - (int)(top >> 23) : 0;
+          const float up = pow2_of_byte(127 + turn);
+          scale *= pow2_of_byte(127 - turn);
+#pragma unroll
+          for (int i = 0; i < G; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[i][j] *= up;
+        }
+#pragma unroll
+        for (int i = 0; i < G; ++i) query_terms<NQ>(x[i], q[i]);
+      }
     }
     // one step is under way while another is added up, and the places of the next are looked up meanwhile
     for (; base + 2 * step < r.hi; base += 2 * step) {
