@@ -513,7 +513,7 @@ def beam_search(model, prompts: Sequence[Sequence[int]], beams: int = 4, max_new
     lengths, limits = start.to(dev), torch.tensor(room, device=dev)[:, None]
     logits = logits[torch.arange(N, device=dev), lengths.long() - 1]
     logits = logits[:, None].expand(N, B, V)
-    scores = torch.where(first.to(dev), 0.0, -torch.inf).expand(N, B).contiguous()
+    scores = torch.where(first, 0.0, -torch.inf).float().to(dev).expand(N, B).contiguous()
     ended = torch.zeros(N, B, dtype=torch.bool, device=dev)
     text = torch.zeros(N, B, steps, dtype=torch.long, device=dev)
     grown = torch.zeros(N, B, dtype=torch.long, device=dev)  # tokens of a beam, up to its end
