@@ -366,12 +366,17 @@ constexpr int kFewLogits = 2048, kFewBeams = 16, kFewKept = 32;
 
 // Small vocabularies in one launch: a workgroup a group, a wave a beam, 32 logits
 // to a lane.  The bound is taken from the beams' scores at once: the K-th largest
-// of the maxima of 64 sets, each a lane of every beam.
+// of the maxima of 64 sets, each a lane of every beam, 13 further on in each: a lane
+// holds neighbouring logits, so a short row fills a few lanes only, and a set that
+// none fills bounds nothing.
 //
 // Takes what saves a launch and a round trip of candidates, us a call, here / in two
 // launches: N1 B4 V2048 K4 6.8 / 10.6, N1 B16 V2048 K16 13.1 / 12.6 (one CU's sums),
 // N64 B16 V2048 K32 18.5 / 22.6, N512 B16 K16 32 / 69.  Larger vocabularies need
-// more registers than sixteen waves have.
+// more registers than sixteen waves have (fewer beams would leave room for some).
+// Twice as many sets as are kept have to be filled, or rows be so short that all
+// candidates are few (us, N64 bf16 K32: B1 V250 78 / 17, B2 V250 23 / 20, B16 V200
+// 20 / 22; sets of the same lanes in each beam took 1013 there).
 template <typename T>
 __global__ void __launch_bounds__(64 * kFewBeams) beam_few(BeamParams p, GroupGeometry g) {
   constexpr int kVec = 16 / sizeof(T), kOwn = kFewLogits / 64;
@@ -417,7 +422,7 @@ __global__ void __launch_bounds__(64 * kFewBeams) beam_few(BeamParams p, GroupGe
   head[b][lane] = reads ? (float)((double)own - (double)most + base) : (float)end.c;
   __syncthreads();
   float of_set = -INFINITY;
-  for (int w = 0; w < p.B; ++w) of_set = fmaxf(of_set, head[w][lane]);
+  for (int w = 0; w < p.B; ++w) of_set = fmaxf(of_set, head[w][(lane + 13 * w) & 63]);
   const float least = kth_of_wave<1>({order_bits(of_set)}, p.K);
   // f for each candidate of this lane
   auto each = [&](auto f) {
@@ -597,7 +602,8 @@ int beam_spans_of(int64_t V) { return (int)((V + kSpan - 1) / kSpan); }
 int launch_beam(const BeamParams& p, hipStream_t st, hipError_t* err) {
   const int lists = p.B * p.spans;
   GroupGeometry g = {fast_div(lists), fast_div(p.spans), fast_div(p.V), 1, 8192 / lists};
-  if (p.V <= kFewLogits && p.B <= kFewBeams && p.K <= kFewKept) {
+  const int64_t filled = p.B * ((p.V * (p.x.dt == TENSION_F32 ? 4 : 2) + 15) / 16);  // lanes, of all beams
+  if (p.V <= kFewLogits && p.B <= kFewBeams && p.K <= kFewKept && (p.V <= 128 || filled >= 2 * p.K)) {
     const unsigned n = (unsigned)p.N, threads = 64 * (unsigned)p.B;
     if (p.x.dt == TENSION_F32) beam_few<float><<<n, threads, 0, st>>>(p, g);
     else if (p.x.dt == TENSION_F16) beam_few<f16><<<n, threads, 0, st>>>(p, g);
