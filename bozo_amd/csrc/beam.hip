@@ -138,12 +138,12 @@ constexpr int kPer = kSpan / kThreads, kMost = 1024;
 // on each thread is a group), which are put in order by counting what is before
 // each.  Where more than kMost do (equal logits) they are taken out one by one.
 //
-// 512 rows of 32768 bf16 logits: 18.4 us in a trace, 1.8 TB/s.  No one thing bounds
-// it: loads, maximum, bound, sums (19 instructions a logit, fourteen of them on 64
-// bits: 8 us of issue) and order follow each other in a workgroup, and five waves
-// a SIMD hide a part of each.  Exponentials without the table, by a polynomial of
-// degree 11, took 0.9 us more, float32 ones 3.5, halved spans or twice the threads
-// more as well.
+// 512 rows of 32768 bf16 logits: 18.6 us in a trace, 1.8 TB/s.  Loads, maximum,
+// bound, sums and order follow each other in a workgroup, and five waves a SIMD hide
+// a part of each: vector instructions, 19 a logit of them for the sums (fourteen on
+// 64 bits), issue in 16% of a wave's cycles.  Exponentials without the table, by a
+// polynomial of degree 11, took 0.9 us more, float32 ones 3.5, halved spans or twice
+// the threads more as well.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) beam_spans(BeamParams p) {
   constexpr int kVec = 16 / sizeof(T);
@@ -299,7 +299,12 @@ struct Candidate {
   uint64_t rank;
 };
 __device__ __forceinline__ bool before(const Candidate& a, const Candidate& b) {
-  return a.c > b.c || (a.c == b.c && a.rank > b.rank);
+  return (a.c > b.c) | ((a.c == b.c) & (a.rank > b.rank));  // both loads at once
+}
+// The first of a candidate and another, by values: chosen by branches they lay in memory.
+__device__ __forceinline__ Candidate first_of(const Candidate& a, double c, uint64_t rank) {
+  const bool other = (c > a.c) | ((c == a.c) & (rank > a.rank));
+  return {other ? c : a.c, other ? rank : a.rank};
 }
 __device__ __forceinline__ uint64_t rank_of(int b, uint64_t key) {
   return (uint64_t)(63 - b) << 52 | key >> 32 << 20 | (key & 0xfffff);
@@ -352,12 +357,11 @@ __device__ __forceinline__ void put_best(const BeamParams& p, const GroupGeometr
 __device__ __forceinline__ Candidate best_of_block(Candidate mine, Candidate* best, int waves) {
 #pragma unroll
   for (int m = 32; m; m >>= 1) {
-    const Candidate o = {__shfl_xor(mine.c, m), shfl64(mine.rank, (threadIdx.x & 63) ^ m)};
-    mine = before(o, mine) ? o : mine;
+    mine = first_of(mine, __shfl_xor(mine.c, m), shfl64(mine.rank, (threadIdx.x & 63) ^ m));
   }
   if ((threadIdx.x & 63) == 0) best[threadIdx.x >> 6] = mine;
   __syncthreads();
-  for (int w = 0; w < waves; ++w) mine = before(best[w], mine) ? best[w] : mine;
+  for (int w = 0; w < waves; ++w) mine = first_of(mine, best[w].c, best[w].rank);
   __syncthreads();
   return mine;
 }
@@ -371,12 +375,12 @@ constexpr int kFewLogits = 2048, kFewBeams = 16, kFewKept = 32;
 // none fills bounds nothing.
 //
 // Takes what saves a launch and a round trip of candidates, us a call, here / in two
-// launches: N1 B4 V2048 K4 6.8 / 10.6, N1 B16 V2048 K16 13.1 / 12.6 (one CU's sums),
-// N64 B16 V2048 K32 18.5 / 22.6, N512 B16 K16 32 / 69.  Larger vocabularies need
-// more registers than sixteen waves have (fewer beams would leave room for some).
+// launches: N1 B4 V2048 K4 7.0 / 11.9, N1 B16 V2048 K16 12.2 / 12.1 (one CU's sums),
+// N64 B16 V2048 K32 16.3 / 18.2, N512 B16 K16 32 / 67.  More than 2048 logits a wave
+// need more registers than sixteen waves have (fewer beams would leave room for some).
 // Twice as many sets as are kept have to be filled, or rows be so short that all
-// candidates are few (us, N64 bf16 K32: B1 V250 78 / 17, B2 V250 23 / 20, B16 V200
-// 20 / 22; sets of the same lanes in each beam took 1013 there).
+// candidates are few (N64 bf16 K32: B1 V250 31 / 16, B2 V250 15 / 16, B16 V200 16 / 22;
+// with the same lanes of each beam in a set 1013 there).
 template <typename T>
 __global__ void __launch_bounds__(64 * kFewBeams) beam_few(BeamParams p, GroupGeometry g) {
   constexpr int kVec = 16 / sizeof(T), kOwn = kFewLogits / 64;
@@ -440,18 +444,29 @@ __global__ void __launch_bounds__(64 * kFewBeams) beam_few(BeamParams p, GroupGe
     if (i < kCandidates) found[i] = c;
   });
   __syncthreads();
-  if (count <= kCandidates) {
+  // Counting what is before each takes 25 ns a comparison of all threads, a round of taking out the best 4 us.
+  if (count <= kCandidates && (count + 64 * p.B - 1) / (64 * p.B) * count <= 128 * p.K) {
     put_best(p, g, found, count, 64 * p.B);
     return;
   }
-  Candidate last = {INFINITY, 0};
-  for (int k = 0; k < p.K; ++k) {  // equal scores: the best is taken out K times
-    Candidate mine = {-INFINITY, 0};
-    each([&](Candidate c) {
-      if (before(last, c) && before(c, mine)) mine = c;
-    });
-    last = best_of_block(mine, best, p.B);
-    if (tid == 0) put(p, k, last);
+  // Many equal scores: the best is taken out K times, and the next of its beam's logits stands in.
+  uint64_t key = ~0ull;
+  Candidate first = {-INFINITY, 0}, mine = end;
+  for (int k = 0; k < p.K; ++k) {
+    if (reads && (k == 0 || first.rank == mine.rank)) {
+      uint64_t next = 0;
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i) {
+        const uint64_t o = x[i] > -INFINITY ? order_key(x[i], (unsigned)index(i)) : 0;
+        if (o < key && o > next) next = o;
+      }
+      key = wave_most(next);
+      mine = Candidate{key ? (double)key_logit(key) - (double)most + base : -INFINITY, key ? rank_of(b, key) : 0};
+    } else if (first.rank == mine.rank) {
+      mine = Candidate{-INFINITY, 0};
+    }
+    first = best_of_block(mine, best, p.B);
+    if (tid == 0) put(p, k, first);
   }
 }
 
@@ -460,7 +475,7 @@ __global__ void __launch_bounds__(64 * kFewBeams) beam_few(BeamParams p, GroupGe
 // which keeps the order) is a bound that few more than the K best reach, and
 // those are put in order by counting what is before each.  A group takes ranks
 // 13 lists apart, so that neither the first ranks of all lists nor a good beam's
-// lists share one.  Bound by its chain: keys, sums, maxima, order (6.6 us for 32
+// lists share one.  Bound by its chain: keys, sums, maxima, order (5.4 us for 32
 // lists of 16).
 __global__ void __launch_bounds__(kThreads) beam_groups(BeamParams p, GroupGeometry g) {
   __shared__ Candidate found[kCandidates];
@@ -513,7 +528,7 @@ __global__ void __launch_bounds__(kThreads) beam_groups(BeamParams p, GroupGeome
 // The same for more lists than that: a list's first threads' ranks are read as
 // far as they reach the bound, the K-th largest of 256 sets' maxima over the
 // lists' first ranks (8192 candidates).  Where more than kCandidates reach it (equal scores) the
-// best is taken out K times.  A call of 64 beams, 131072 logits, K 64: 43 us (a
+// best is taken out K times.  A call of 64 beams, 131072 logits, K 64: 38 us (a
 // merge of the lists' heads by one wave: 511).
 __global__ void __launch_bounds__(kManyThreads) beam_groups_many(BeamParams p, GroupGeometry g) {
   constexpr int kWaves = kManyThreads / 64, kDeep = 4, kSets = 256;
@@ -586,7 +601,7 @@ __global__ void __launch_bounds__(kManyThreads) beam_groups_many(BeamParams p, G
   for (int k = 0; k < p.K; ++k) {
     Candidate mine = {-INFINITY, 0};
     walk(p.K, [&](Candidate x, int) {
-      if (before(last, x) && before(x, mine)) mine = x;
+      mine = first_of(mine, before(last, x) ? x.c : -INFINITY, x.rank);
       return true;
     });
     mine = best_of_block(mine, best, kWaves);

@@ -148,3 +148,26 @@ def test_short_rows(B, V, K, dt):
         assert np.array_equal(tok, wt) and np.array_equal(par, wp)
     full = torch.randn(3, B, 2048, generator=g, device="cuda").to(dt)
     assert microseconds(x, s, K) <= 25 * microseconds(full, s, K)
+
+
+@pytest.mark.parametrize("B,V,K", [(1, 2048, 4), (1, 2048, 1), (2, 2000, 32), (4, 500, 8), (4, 2048, 32), (16, 2048, 32), (16, 128, 32), (7, 777, 5),
+                                   (16, 2049, 32), (3, 8192, 64), (64, 20000, 64)])
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_many_equal_scores(B, V, K, dt):
+    """Rows of one value, or of three; beams at their end, beams that run out of tokens: right, and no slower by orders."""
+    g = torch.Generator(device="cuda").manual_seed(V + B)
+    zeros = torch.zeros(2, B, V, device="cuda", dtype=dt)
+    few = torch.randint(0, 3, (2, 1, V), generator=g, device="cuda").to(dt).expand(2, B, V).contiguous()
+    few[:, :, ::5] *= -0.0
+    scores = torch.zeros(2, B, device="cuda")
+    scores[1] = -0.25 * (torch.arange(B, device="cuda") % 3)
+    ended = torch.rand(2, B, generator=g, device="cuda") < 0.3
+    out_of = few.clone()
+    out_of[:, 0, 3:] = -math.inf
+    out_of[0, B // 2, 1:] = -math.inf
+    for x in (zeros, few, out_of):
+        for e in (None, ended):
+            (out, tok, par), (want, wt, wp) = select(x, scores, K, e, V // 2)
+            assert np.array_equal(tok, wt) and np.array_equal(par, wp)
+    usual = torch.randn(2, B, V, generator=g, device="cuda").to(dt)
+    assert max(microseconds(zeros, scores, K), microseconds(few, scores, K)) <= 25 * microseconds(usual, scores, K)
