@@ -993,9 +993,10 @@ int tension_paged_reorder(const tension_paged* layers, int32_t count, int32_t* o
     } else if (c.P != p.P || c.S != p.S || c.table_len != p.len) {
       return fail(TENSION_ERR_ARG, "paged reorder: layers of different pages, page sizes or tables");
     }
-    // bytes of a page's rows of all heads, as a workgroup counts them
-    if (mul_cap(mul_cap(Hk, c.S, 1 << 30), 4 * D, 1 << 30) < 0)
-      return fail(TENSION_ERR_ARG, "paged reorder: pages of more than 2^30 bytes");
+    // a workgroup counts the bytes of a page's rows of all heads, four a value at most
+    if (mul_cap(mul_cap(Hk, c.S, 1 << 28), D, 1 << 28) < 0)
+      return fail(TENSION_ERR_ARG, "paged reorder: pages of more than 2^28 values: Hk=%lld page_size=%d D=%lld", (long long)Hk,
+                  c.S, (long long)D);
   }
   if (out_table == p.table) return fail(TENSION_ERR_ARG, "paged reorder: out_table must be another buffer");
   for (int i = 0; i < count; i += kReorderLayers) {

@@ -377,7 +377,7 @@ def paged_reorder(layers: Sequence[PagedKV], table: Tensor, lengths: Tensor, par
     beam that nobody goes on from, into whose first the parent's tokens are copied
     in every layer (the pages are written in place).  So each beam needs a page of
     its own for the tokens behind the last full page, and no other beam's row may
-    name it."""
+    name it.  At most 4096 layers, 254200 beams and 2^28 values a page."""
     ls = [tuple(kv) for kv in layers]
     args = (*([kv[i] for kv in ls] for i in range(4)), table, lengths, parents)
     out = L.host().paged_reorder(*args)

@@ -482,7 +482,8 @@ int tension_paged_plan(int32_t* table, int64_t table_stride, int64_t table_len,
  *   lengths[n] / S, whose pages are full, are the parent's.  The others are the
  *   parent's for the first beam that goes on from it; each further one takes
  *   those of a beam that nobody goes on from (in order), and if lengths[n] % S
- *   tokens lie in the first of them, they are copied there, in every layer. */
+ *   tokens lie in the first of them, they are copied there, in every layer.
+ *   count <= 4096, N * B <= 254200, and Hk * page_size * D <= 2^28. */
 int tension_paged_reorder(const tension_paged* layers, int32_t count,
                           int32_t* out_table, int64_t out_stride,
                           const int32_t* lengths, const int64_t* parents,
