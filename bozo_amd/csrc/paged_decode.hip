@@ -163,13 +163,16 @@ void launch_join(const PagedDecodeParams& p, hipStream_t st) {
 // Tried: one split, and what gives each CU one to four workgroups (two where
 // the matrix kernel holds head dim 128), with 128 keys to a split at least.
 //   Rows of 4-bit pages are a quarter of that, and a CU by itself streams no
-// more of them than its share of all (24 KB/us; the matrix kernel, which takes
-// sixteen query heads through tau whatever their number, 17 at D64, 20 at D128).
+// more of them than its share of all (24 KB/us, the vector kernel's at D64; the
+// matrix kernel, which takes sixteen query heads through tau whatever their number,
+// reaches 17 at D64 and 20 at D128, and is counted alike).
 void paged_decode_split(int64_t N, int64_t H, int64_t Hk, int64_t D, int64_t keys, bool fp4, int* splits, int* chunk) {
   constexpr float kAllBytesPerUs = 23e3f;
   const float kCuBytesPerUs = fp4 ? 24e3f : 49e3f, kJoinUs = fp4 ? 5.f : 3.5f;
   constexpr int64_t kLeast = 128, kMostGroups = ((int64_t)1 << 22) - 1;
-  // 4-bit pages that the matrix kernel has no head dim for are read once for each query head
+  // 4-bit pages that the matrix kernel has no head dim for are read once for each query head.  So are those that it does
+  // not take for other reasons (page sizes not in sixteens, rows or exponents that lie otherwise, no more query heads than
+  // CUs): they are counted as shared all the same, and get more splits than their bytes alone would.
   const int64_t rows = fp4 && (D % 32 || D > 128) ? N * H : N * Hk, cus = device_cus();
   const float row_bytes = (float)keys * (float)(fp4 ? D : 4 * D);
   const float all_us = (float)rows * row_bytes / (kAllBytesPerUs * (float)cus);
